@@ -404,6 +404,123 @@ int mzs_replay_update_value(int32_t batch, int32_t num_unroll, double* const* ro
                             const int32_t* game_len, const int64_t* game_idx, const int64_t* pos,
                             const double* new_value, double* prio_game);
 
+/* ---- policy rows: log-probabilities, entropy, alternatives, gradient ----------------------------
+ * What evaluate_loss takes of a policy head (the cross-entropy term, muzero_model.py:690-700), for any number
+ * of actions — a Box action space is the cartesian product of `bins` samples per dimension
+ * (muzero_model.py:994-1051) — and for reading policies back (Game.policy_step's distribution, game.py:176-225).
+ * For each row of logits l, with z_i = l_i * inverse_temperature, z_i = -inf where the mask forbids action i:
+ *     log_z = log sum_i exp z_i       log_prob = z_action - log_z       entropy = -sum_i p_i log p_i,  p_i = exp(z_i - log_z)
+ *     top alternatives: the `top` largest logits, ties to the lower index, their log-probabilities
+ * and with the row's upstream coefficients g_a (of log_prob), g_h (of entropy), g_z (of log_z):
+ *     grad_i = inverse_temperature * (p_i (g_z - g_a - g_h (log p_i + entropy)) + [i = action] g_a)
+ * A row that allows nothing (all masked or -inf): log_z = log_prob = -inf, entropy 0, gradient 0, no alternatives.
+ * Action < 0: the row has none (log_prob 0, g_a not used).  Action >= n_actions: log_prob NaN.  Action forbidden:
+ * log_prob -inf, and its own gradient element stays 0.  A NaN or +inf among the allowed logits makes the row's values and
+ * gradient NaN (alternatives: NaN ranks first); masked logits are never looked at.  Slots of alternatives beyond the allowed
+ * actions hold index -1 and -inf.
+ * Everything is computed in fp32; logits and gradient are fp32, bf16 or fp16. */
+#define MZS_DTYPE_FLOAT 0
+#define MZS_DTYPE_BFLOAT 1
+#define MZS_DTYPE_HALF 2
+#define MZS_POLICY_MAX_TOP 32
+
+typedef struct mzs_policy_args {
+    int32_t device;             /* HIP device of every pointer below                                  */
+    int32_t dtype;              /* MZS_DTYPE_* of logits and grad_logits                              */
+    int64_t rows;
+    int64_t n_actions;          /* 1 .. 2^31 - 1                                                      */
+    const void* logits;         /* [rows][n_actions], a row every logits_stride elements (0: one row for all) */
+    int64_t logits_stride;
+    const uint8_t* mask;        /* 1 = allowed; a row every mask_stride bytes (0: one mask for all rows); NULL: all allowed */
+    int64_t mask_stride;
+    const void* action;         /* [rows], or NULL: no actions                                        */
+    int32_t action_bytes;       /* 4 (int32) or 8 (int64)                                             */
+    int32_t top;                /* alternatives per row, 0 .. MZS_POLICY_MAX_TOP                      */
+    float inverse_temperature;  /* > 0                                                                */
+    float* log_prob;            /* [rows]                                                             */
+    float* entropy;             /* [rows]                                                             */
+    float* log_z;               /* [rows]                                                             */
+    float* row_stats;           /* [rows][2]: largest allowed logit, sum of exponentials relative to it: what the
+                                   gradient reads back instead of log_z, which rounds away the low bits of large logits */
+    float* top_log_prob;        /* [rows][top]                                                        */
+    int32_t* top_action;        /* [rows][top]                                                        */
+    const float* grad_log_prob; /* [rows] or NULL (0)                                                 */
+    const float* grad_entropy;  /* [rows] or NULL (0)                                                 */
+    const float* grad_log_z;    /* [rows] or NULL (0)                                                 */
+    void* grad_logits;          /* [rows][n_actions], a row every grad_stride elements; may be `logits` itself (same stride) */
+    int64_t grad_stride;
+    void* workspace;            /* mzs_policy_workspace bytes, 16-byte aligned, this call's alone     */
+    size_t workspace_bytes;
+} mzs_policy_args;
+
+/* bytes of workspace the three calls below need for these sizes (0: none) */
+int mzs_policy_workspace(const mzs_policy_args* args, size_t* bytes_out);
+/* writes log_prob, entropy, log_z, row_stats and, with top > 0, the alternatives */
+int mzs_policy_log_probs(const mzs_policy_args* args, void* stream);
+/* writes grad_logits from row_stats and entropy of an earlier mzs_policy_log_probs on the same logits, mask and temperature */
+int mzs_policy_log_probs_grad(const mzs_policy_args* args, void* stream);
+/* both at once, for upstream coefficients known beforehand: reads the logits once where a row fits on chip */
+int mzs_policy_log_probs_train(const mzs_policy_args* args, void* stream);
+
+/* ---- optimizer over many tensors: global gradient norm, AdamW step --------------------------------
+ * What stands beside Adam / SGD (init_criterion_and_optimizer, muzero_model.py:418-421) for parameter lists of any
+ * length and type: one call walks every tensor.  Tensors are named by a table in device memory; the states are flat
+ * buffers in which tensor i occupies its count of elements from state_at(i) on, state_at(0) = 0 and
+ * state_at(i + 1) = state_at(i) + count(i) rounded up to MZS_OPTIM_ALIGN. */
+#define MZS_OPTIM_ALIGN 64       /* elements between the starts of two tensors' states, a multiple of       */
+#define MZS_OPTIM_BLOCK 32       /* 8-bit states: elements that share one exponent                          */
+#define MZS_OPTIM_ENTRY_BYTES 32 /* device table: bytes per tensor (one more entry behind the last)         */
+#define MZS_OPTIM_CONTROL_BYTES 64
+
+/* Writes the table of n tensors to table_dev ((n + 1) * MZS_OPTIM_ENTRY_BYTES bytes, 16-byte aligned): tensor i has counts[i]
+ * elements from pointers[i] on (device memory, contiguous; NULL: no tensor — a parameter without a gradient).
+ * Runs on the stream from values copied at the call (the host arrays may go afterwards); *n_tiles_out = the tiles a kernel walks. */
+int mzs_optim_table(int32_t device, int32_t n, const void* const* pointers, const int64_t* counts, void* table_dev,
+                    int64_t* n_tiles_out, void* stream);
+
+/* bytes of workspace for a norm over n_tiles tiles (zeroed once by nobody: its contents are written before they are read) */
+size_t mzs_grad_norm_workspace(int64_t n_tiles);
+
+/* norm_dev[0] = grad_scale * sqrt(sum of squares over every tensor of the table), summed in fp64 in a fixed order.
+ * dtype: MZS_DTYPE_* of all tensors. */
+int mzs_grad_norm(int32_t device, int32_t n, const void* table_dev, int64_t n_tiles, int32_t dtype, double grad_scale,
+                  float* norm_dev, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One AdamW step (decoupled weight decay) of every tensor:
+ *     g' = clip * grad_scale * g          clip = min(1, max_norm / (norm + 1e-6)), 1 without max_norm
+ *     m = beta1 m + (1 - beta1) g'        v = beta2 v + (1 - beta2) g'^2
+ *     w = w (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * all in fp32.  t is the device's own step counter (control_dev), so a captured step replays as the next one.  With
+ * max_norm > 0 a norm that is not finite skips the step: nothing is written but the skip counter.
+ * state_bits 32: exp_avg = m, exp_avg_sq = v, fp32.
+ * state_bits 8: m and u = sqrt(v) as e4m3 codes (OCP fp8, bytes) with one e8m0 exponent byte per 32 elements (the smallest power of two
+ *   that brings the block's largest magnitude to 448 at most), rounded to a neighbouring code by dither: element k
+ *   of the flat state goes up where the fraction it lies above the lower code exceeds 1 - r / 65536, r = 16 bits of a hash of (seed, t, k);
+ *   an u > 0 keeps at least the smallest code, so that v never becomes 0 under an m that is not.
+ * master != NULL: the fp32 weights (a flat buffer like the states), w is read and written there and params only written. */
+typedef struct mzs_adamw_args {
+    int32_t device, n;               /* tensors                                                        */
+    int64_t n_tiles;                 /* of the parameter table                                         */
+    int32_t param_dtype, grad_dtype; /* MZS_DTYPE_*                                                    */
+    int32_t state_bits;              /* 32 or 8                                                        */
+    int32_t norm_given;              /* 1: norm_dev holds the norm to clip by; 0: computed here when max_norm > 0 */
+    const void* params_table;        /* mzs_optim_table                                                */
+    const void* grads_table;         /* mzs_optim_table, the same counts                               */
+    float* master;                   /* or NULL                                                        */
+    void* exp_avg;                   /* fp32 or e4m3 codes                                             */
+    void* exp_avg_sq;                /* fp32 v, or the e4m3 codes of its root                          */
+    uint8_t* exp_avg_exponent;       /* state_bits 8: e8m0 bytes, one per 32 elements                  */
+    uint8_t* exp_avg_sq_exponent;
+    int32_t* control_dev;            /* MZS_OPTIM_CONTROL_BYTES: [0] steps taken, [1] steps skipped; the rest is the step's own */
+    float* norm_dev;                 /* the norm (written unless norm_given); may be NULL without max_norm */
+    const float* lr_dev;             /* or NULL: lr                                                    */
+    double lr, beta1, beta2, eps, weight_decay, max_norm, grad_scale;
+    uint64_t seed;
+    void* workspace;                 /* mzs_grad_norm_workspace(n_tiles) bytes when the norm is computed here */
+    size_t workspace_bytes;
+} mzs_adamw_args;
+int mzs_adamw_step(const mzs_adamw_args* args, void* stream);
+
 const char* mzs_last_error(void);
 const char* mzs_version(void);
 

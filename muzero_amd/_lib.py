@@ -47,6 +47,34 @@ class Config(C.Structure):
                 ("root_exploration_fraction", C.c_double), ("pbc_table", C.c_void_p)]
 
 
+DTYPE_FLOAT, DTYPE_BFLOAT, DTYPE_HALF = 0, 1, 2
+POLICY_MAX_TOP = 32
+OPTIM_ALIGN, OPTIM_BLOCK, OPTIM_ENTRY_BYTES, OPTIM_CONTROL_BYTES = 64, 32, 32, 64
+
+
+class PolicyArgs(C.Structure):
+    _fields_ = [("device", C.c_int32), ("dtype", C.c_int32), ("rows", C.c_int64), ("n_actions", C.c_int64),
+                ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+                ("action", C.c_void_p), ("action_bytes", C.c_int32), ("top", C.c_int32),
+                ("inverse_temperature", C.c_float), ("log_prob", C.c_void_p), ("entropy", C.c_void_p),
+                ("log_z", C.c_void_p), ("row_stats", C.c_void_p), ("top_log_prob", C.c_void_p),
+                ("top_action", C.c_void_p), ("grad_log_prob", C.c_void_p), ("grad_entropy", C.c_void_p),
+                ("grad_log_z", C.c_void_p), ("grad_logits", C.c_void_p), ("grad_stride", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class AdamWArgs(C.Structure):
+    _fields_ = [("device", C.c_int32), ("n", C.c_int32), ("n_tiles", C.c_int64), ("param_dtype", C.c_int32),
+                ("grad_dtype", C.c_int32), ("state_bits", C.c_int32), ("norm_given", C.c_int32),
+                ("params_table", C.c_void_p), ("grads_table", C.c_void_p), ("master", C.c_void_p),
+                ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("exp_avg_exponent", C.c_void_p),
+                ("exp_avg_sq_exponent", C.c_void_p), ("control_dev", C.c_void_p), ("norm_dev", C.c_void_p),
+                ("lr_dev", C.c_void_p), ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("eps", C.c_double), ("weight_decay", C.c_double), ("max_norm", C.c_double),
+                ("grad_scale", C.c_double), ("seed", C.c_uint64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
 _SIGNATURES = {
     "mzs_create": (C.c_int, [C.POINTER(Config), C.POINTER(C.c_void_p)]),
     "mzs_destroy": (None, [C.c_void_p]),
@@ -114,6 +142,16 @@ _SIGNATURES = {
                                               C.c_void_p]),
     "mzs_replay_update_value": (C.c_int, [C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                           C.c_void_p, C.c_void_p, C.c_void_p]),
+    "mzs_policy_workspace": (C.c_int, [C.POINTER(PolicyArgs), C.POINTER(C.c_size_t)]),
+    "mzs_policy_log_probs": (C.c_int, [C.POINTER(PolicyArgs), C.c_void_p]),
+    "mzs_policy_log_probs_grad": (C.c_int, [C.POINTER(PolicyArgs), C.c_void_p]),
+    "mzs_policy_log_probs_train": (C.c_int, [C.POINTER(PolicyArgs), C.c_void_p]),
+    "mzs_optim_table": (C.c_int, [C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(C.c_int64),
+                                  C.c_void_p]),
+    "mzs_grad_norm_workspace": (C.c_size_t, [C.c_int64]),
+    "mzs_grad_norm": (C.c_int, [C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_double, C.c_void_p,
+                                C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mzs_adamw_step": (C.c_int, [C.POINTER(AdamWArgs), C.c_void_p]),
     "mzs_last_error": (C.c_char_p, []),
     "mzs_version": (C.c_char_p, []),
 }

@@ -33,6 +33,7 @@
 #include "mzs_selfplay.h"
 #include "mzs_replay.h"
 #include "mzs_vision_train.h"
+#include "mzs_error.h"
 
 using namespace mzs;
 
@@ -1176,6 +1177,15 @@ void fill_search_params(mzs_handle* h, SearchParams* p, int n_games, int S, int 
 }
 
 }  // namespace
+
+int mzs::set_error(int code, const char* text) noexcept {
+    try {
+        g_err = text;
+    } catch (...) {
+        g_err.clear();
+    }
+    return code;
+}
 
 extern "C" {
 
