@@ -16,7 +16,9 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kTile = 4096;       /* elements of a tile */
 constexpr int kFillEntries = 120; /* table entries a launch carries in its arguments */
-constexpr int kMaxPartials = 1024;
+constexpr int kMaxPartials = 2048; /* 8 blocks on each of 256 CUs */
+constexpr int kVec = 4;           /* elements a thread takes at once */
+constexpr int kStep = kBlock * kVec;
 constexpr int kGroup = MZS_OPTIM_BLOCK;
 
 struct Entry {
@@ -40,22 +42,62 @@ __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(bf16 v) { return __uint_as_float((uint32_t)v.bits << 16); }
 __device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(bf16* p, float v) { /* nearest even; a NaN stays one */
-    uint32_t b = __float_as_uint(v);
-    b = v != v ? 0x7fc00000u : b + 0x7fffu + ((b >> 16) & 1u);
-    p->bits = (uint16_t)(b >> 16);
+__device__ __forceinline__ uint32_t bf16_bits(float v) { /* nearest even; a NaN stays one */
+    const uint32_t b = __float_as_uint(v);
+    return v != v ? 0x7fc0u : (b + 0x7fffu + ((b >> 16) & 1u)) >> 16;
 }
+__device__ __forceinline__ void put(bf16* p, float v) { p->bits = (uint16_t)bf16_bits(v); }
 __device__ __forceinline__ void put(_Float16* p, float v) { *p = (_Float16)v; }
 
-/* the tensor that tile `tile` is of: the last entry with first_tile <= tile (empty tensors have no tiles) */
-__device__ __forceinline__ int find_tensor(const Entry* __restrict__ table, int n, int64_t tile) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (table[mid].first_tile <= tile) lo = mid;
-        else hi = mid;
+/* four (or eight) consecutive elements in one access; tensors may start at any element, which costs the hardware nothing from 4 bytes on */
+typedef uint32_t w2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t w4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float low_half(uint32_t v, bf16) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float high_half(uint32_t v, bf16) { return __uint_as_float(v & 0xffff0000u); }
+__device__ __forceinline__ float low_half(uint32_t v, _Float16) { return (float)__builtin_bit_cast(h2, v).x; }
+__device__ __forceinline__ float high_half(uint32_t v, _Float16) { return (float)__builtin_bit_cast(h2, v).y; }
+__device__ __forceinline__ uint32_t pack_halves(float a, float b, bf16) { return bf16_bits(a) | (bf16_bits(b) << 16); }
+__device__ __forceinline__ uint32_t pack_halves(float a, float b, _Float16) {
+    return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
+}
+template <typename T>
+struct Quad { /* as it comes from memory */
+    w2 raw;
+    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const w2*>(p); }
+    __device__ __forceinline__ float get(int j) const {
+        const uint32_t v = j < 2 ? raw.x : raw.y;
+        return j & 1 ? high_half(v, T()) : low_half(v, T());
     }
-    return lo;
+    static __device__ __forceinline__ void store(T* p, const float* v) {
+        *reinterpret_cast<w2*>(p) = w2{pack_halves(v[0], v[1], T()), pack_halves(v[2], v[3], T())};
+    }
+};
+template <>
+struct Quad<float> {
+    f4 raw;
+    __device__ __forceinline__ void load(const float* p) { raw = *reinterpret_cast<const f4*>(p); }
+    __device__ __forceinline__ float get(int j) const { return raw[j]; }
+    static __device__ __forceinline__ void store(float* p, const float* v) {
+        *reinterpret_cast<f4*>(p) = f4{v[0], v[1], v[2], v[3]};
+    }
+};
+
+/* The tensor that tile `tile` is of: the last entry with first_tile <= tile (empty tensors have no tiles).  The lanes of a wave look at
+ * 64 entries at once: two dependent loads for 4096 tensors instead of twelve. */
+__device__ __forceinline__ int find_tensor(const Entry* __restrict__ table, int n, int64_t tile) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, len = n;
+    while (len > 1) {
+        const int s = (len + 63) >> 6;
+        const int at = lane * s;
+        const bool before = at < len && table[lo + at].first_tile <= tile;
+        const int hit = __popcll(__ballot(before)) - 1; /* lane 0's entry is always one */
+        lo += hit * s;
+        len = len - hit * s < s ? len - hit * s : s;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
 }
 
 /* fixed-order sum over the block; the total in thread 0 */
@@ -69,21 +111,62 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
     return lds[0];
 }
 
+/* squares of elements [from, to) of one tensor, this thread's share, in fp64 (fp32 squares overflow from 1.8e19 on and vanish
+ * below 1e-23; the fp64 fma runs at the fp32 rate here, so the loads bound it either way) */
+template <typename G>
+__device__ __forceinline__ double sum_squares(const G* __restrict__ g, int64_t from, int64_t to, int threads) {
+    constexpr int kUnroll = 4;
+    constexpr int kWide = sizeof(G) == 4 ? 4 : 8; /* 16 bytes */
+    double sum[2] = {0.0, 0.0};
+    int64_t i = from + (int64_t)threadIdx.x * kWide;
+    const int64_t step = (int64_t)threads * kWide;
+    for (; i + (kUnroll - 1) * step + kWide <= to; i += kUnroll * step) {
+        Quad<G> q[kUnroll][kWide / 4];
+        _Pragma("unroll") for (int u = 0; u < kUnroll; ++u) {
+            if constexpr (kWide == 4) {
+                q[u][0].load(g + i + u * step);
+            } else {
+                const w4 raw = *reinterpret_cast<const w4*>(g + i + u * step);
+                q[u][0].raw = w2{raw.x, raw.y}, q[u][1].raw = w2{raw.z, raw.w};
+            }
+        }
+        _Pragma("unroll") for (int u = 0; u < kUnroll; ++u)
+            _Pragma("unroll") for (int j = 0; j < kWide; ++j) {
+                const double x = (double)q[u][j / 4].get(j % 4);
+                sum[j & 1] = fma(x, x, sum[j & 1]);
+            }
+    }
+    for (; i < to; i += step) {
+        const int64_t end = i + kWide < to ? i + kWide : to;
+        for (int64_t k = i; k < end; ++k) {
+            const double x = (double)to_float(g[k]);
+            sum[0] = fma(x, x, sum[0]);
+        }
+    }
+    return sum[0] + sum[1];
+}
+
+/* One read of everything: a block takes a run of consecutive tiles, which is one contiguous range for each tensor it
+ * meets; four 16-byte loads a thread in flight. */
 template <typename G>
 __global__ void __launch_bounds__(kBlock) k_norm_partial(const Entry* __restrict__ table, int n, int64_t n_tiles,
                                                          double* __restrict__ partial) {
     __shared__ double lds[kBlock];
+    const int64_t per = n_tiles / gridDim.x, more = n_tiles % gridDim.x, b = blockIdx.x;
+    int64_t tile = b * per + (b < more ? b : more);
+    const int64_t end = tile + per + (b < more ? 1 : 0);
     double sum = 0.0;
-    for (int64_t tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
-        const Entry e = table[find_tensor(table, n, tile)];
-        if (!e.data) continue;
-        const int64_t from = (tile - e.first_tile) * kTile;
-        const int64_t to = from + kTile < e.count ? from + kTile : e.count;
-        const G* g = static_cast<const G*>(e.data);
-        for (int64_t i = from + threadIdx.x; i < to; i += kBlock) {
-            const double x = (double)to_float(g[i]);
-            sum = fma(x, x, sum);
+    int which = find_tensor(table, n, tile);
+    while (tile < end && which < n) {
+        const Entry e = table[which];
+        const int64_t tiles = (e.count + kTile - 1) / kTile;
+        const int64_t last = e.first_tile + tiles < end ? e.first_tile + tiles : end;
+        if (e.data && last > tile) {
+            const int64_t to = (last - e.first_tile) * kTile;
+            sum += sum_squares(static_cast<const G*>(e.data), (tile - e.first_tile) * kTile, to < e.count ? to : e.count, kBlock);
         }
+        if (last > tile) tile = last;
+        ++which;
     }
     const double total = block_sum(sum, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = total;
@@ -172,33 +255,22 @@ __global__ void __launch_bounds__(kBlock) k_adamw_begin(const StepArgs a) {
     c->inv_root_2 = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
 }
 
-/* ---- 8-bit states: e4m3 codes under a shared power of two */
-__device__ __forceinline__ float code_value(uint8_t code) {
-    const uint32_t mag = code & 0x7fu, e = mag >> 3, f = mag & 7u;
-    float v = e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * 0.001953125f;
-    if (mag == 0x7fu) v = __builtin_nanf("");
-    return (code & 0x80u) ? -v : v;
+/* ---- 8-bit states: e4m3 codes under a shared power of two.  The conversions are the hardware's: its stochastic rounding
+ * with the 16 dither bits in the high half of the random word is floor(|y| / step + r / 65536), subnormal codes included. */
+__device__ __forceinline__ float exponent_value(uint32_t e) { /* 2^(e - 127); 255: NaN */
+    return e == 255u ? __builtin_nanf("") : e ? __uint_as_float(e << 23) : 5.87747175411143754e-39f;
 }
-__device__ __forceinline__ float exponent_value(uint8_t e) { /* 2^(e - 127); 255: NaN */
-    return e == 255 ? __builtin_nanf("") : e ? __uint_as_float((uint32_t)e << 23) : 5.87747175411143754e-39f;
+/* exponent byte of a block whose largest magnitude has these bits: 448 = 1.75 * 2^8, a mantissa above 1.75 carries */
+__device__ __forceinline__ uint32_t block_exponent(uint32_t most) {
+    const int e = (int)((most + 0x1fffffu) >> 23) - 8;
+    return most >= 0x7f800000u ? 255u : (uint32_t)(e < 0 ? 0 : e);
 }
-/* exponent byte of a block whose largest magnitude is `most` */
-__device__ __forceinline__ uint8_t block_exponent(float most) {
-    const uint32_t b = __float_as_uint(most);
-    if (b >= 0x7f800000u) return 255;
-    const int e = (int)((b + 0x1fffffu) >> 23) - 8; /* 448 = 1.75 * 2^8: a mantissa above 1.75 carries */
-    return (uint8_t)(e < 0 ? 0 : e);
-}
-/* |y| <= 448 to a code: the grid point below |y| / step + r steps, r in [0, 1) */
-__device__ __forceinline__ uint8_t to_code(float y, float r) {
-    if (y != y) return 0x7f;
-    const float a = fabsf(y);
-    const int e = (int)(__float_as_uint(a) >> 23) - 127;
-    const int oct = e < -6 ? -6 : e;
-    const float inv_step = __uint_as_float((uint32_t)(127 - (oct - 3)) << 23);
-    int q = (int)floorf(a * inv_step + r); /* 8 .. 16 in a normal octave, 0 .. 8 below */
-    uint32_t code = oct == -6 ? (uint32_t)q : (uint32_t)(((oct + 6) << 3) + q);
-    return (uint8_t)(code | ((__float_as_uint(y) >> 24) & 0x80u));
+/* largest of a lane's value over its eight neighbours' */
+__device__ __forceinline__ uint32_t max_over_8(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true));  /* quad_perm 1 0 3 2 */
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true));  /* quad_perm 2 3 0 1 */
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true)); /* row_half_mirror: the other four */
+    return v;
 }
 
 __device__ __forceinline__ float adamw(float w, float& m, float& v, float& root, float g, const StepArgs& a, const Control& c) {
@@ -206,6 +278,99 @@ __device__ __forceinline__ float adamw(float w, float& m, float& v, float& root,
     v = v * a.b2 + g * g * a.one_minus_b2;
     root = __builtin_sqrtf(v);
     return w * c.decay - c.step_size * (m / (root * c.inv_root_2 + a.eps));
+}
+
+/* a quad's loads and stores; kWhole: all four elements exist, else `count` of them do (tail of a tensor) */
+template <typename T, bool kWhole>
+__device__ __forceinline__ void load_quad(const T* p, int count, float* out) {
+    if (kWhole) {
+        Quad<T> q;
+        q.load(p);
+        _Pragma("unroll") for (int j = 0; j < kVec; ++j) out[j] = q.get(j);
+    } else {
+        _Pragma("unroll") for (int j = 0; j < kVec; ++j) out[j] = j < count ? to_float(p[j]) : 0.0f;
+    }
+}
+template <typename T, bool kWhole>
+__device__ __forceinline__ void store_quad(T* p, int count, const float* v) {
+    if (kWhole) Quad<T>::store(p, v);
+    else _Pragma("unroll") for (int j = 0; j < kVec; ++j) if (j < count) put(p + j, v[j]);
+}
+
+/* One tile: kTile / kStep quads a thread, every load of them issued before the first is used. */
+template <typename P, typename G, bool kBytes, bool kWhole>
+__device__ __forceinline__ void step_tile(const StepArgs& a, const Control& c, P* __restrict__ param, const G* __restrict__ grad,
+                                          int64_t state_at, int count) {
+    constexpr int kUnroll = kWhole ? kTile / kStep : 1;
+    const bool master = a.master != nullptr;
+    for (int i0 = 0; i0 < (kWhole ? kTile : count); i0 += kUnroll * kStep) {
+        float g[kUnroll][kVec], w[kUnroll][kVec], m[kUnroll][kVec], v[kUnroll][kVec];
+        uint32_t mc[kUnroll], vc[kUnroll], me[kUnroll], ve[kUnroll];
+        _Pragma("unroll") for (int u = 0; u < kUnroll; ++u) {
+            const int i = i0 + u * kStep + (int)threadIdx.x * kVec, left = count - i;
+            const int64_t k = state_at + i;
+            load_quad<G, kWhole>(grad + i, left, g[u]);
+            if (master) load_quad<float, kWhole>(a.master + k, left, w[u]);
+            else load_quad<P, kWhole>(param + i, left, w[u]);
+            if (kBytes) { /* codes come in whole blocks: the state is padded, the blocks' zeros behind a tensor stay zeros */
+                mc[u] = vc[u] = me[u] = ve[u] = 0;
+                if (kWhole || left > 0) {
+                    mc[u] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + k);
+                    vc[u] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + k);
+                    me[u] = a.m_exp[k / kGroup], ve[u] = a.v_exp[k / kGroup];
+                }
+            } else {
+                load_quad<float, kWhole>(static_cast<const float*>(a.m) + k, left, m[u]);
+                load_quad<float, kWhole>(static_cast<const float*>(a.v) + k, left, v[u]);
+            }
+        }
+        _Pragma("unroll") for (int u = 0; u < kUnroll; ++u) {
+            const int i = i0 + u * kStep + (int)threadIdx.x * kVec, left = count - i;
+            const int64_t k = state_at + i;
+            float root[kVec];
+            if (kBytes) {
+                const float sm = exponent_value(me[u]), sv = exponent_value(ve[u]);
+                const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[u], false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[u], true);
+                const auto v01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)vc[u], false), v23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)vc[u], true);
+                m[u][0] = m01[0] * sm, m[u][1] = m01[1] * sm, m[u][2] = m23[0] * sm, m[u][3] = m23[1] * sm;
+                const float r[kVec] = {v01[0] * sv, v01[1] * sv, v23[0] * sv, v23[1] * sv};
+                _Pragma("unroll") for (int j = 0; j < kVec; ++j) v[u][j] = r[j] * r[j];
+            }
+            _Pragma("unroll") for (int j = 0; j < kVec; ++j)
+                w[u][j] = adamw(w[u][j], m[u][j], v[u][j], root[j], g[u][j] * c.scale, a, c);
+            if (kBytes) {
+                uint32_t most_m = 0, most_v = 0; /* as bits, so that a NaN is the largest */
+                _Pragma("unroll") for (int j = 0; j < kVec; ++j) if (kWhole || j < left) {
+                    most_m = max(most_m, __float_as_uint(m[u][j]) & 0x7fffffffu);
+                    most_v = max(most_v, __float_as_uint(root[j]) & 0x7fffffffu);
+                }
+                me[u] = block_exponent(max_over_8(most_m)), ve[u] = block_exponent(max_over_8(most_v));
+                const float sm = __uint_as_float((254u - me[u]) << 23), sv = __uint_as_float((254u - ve[u]) << 23);
+                const bool nan_m = me[u] == 255u, nan_v = ve[u] == 255u;
+                uint32_t x = (uint32_t)k * 0x9E3779B1u + c.key;
+                mc[u] = vc[u] = 0;
+                _Pragma("unroll") for (int j = 0; j < kVec; ++j) {
+                    const uint32_t r = mix(x + j * 0x9E3779B1u);
+                    uint32_t cm = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(m[u][j] * sm, (int)(r & 0xffff0000u), 0, 0) & 0xffu;
+                    uint32_t cv = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(root[j] * sv, (int)(r << 16), 0, 0) & 0xffu;
+                    if (cv == 0 && root[j] > 0.0f) cv = 1;
+                    if (nan_m) cm = 0x7f;
+                    if (nan_v) cv = 0x7f;
+                    if (kWhole || j < left) mc[u] |= cm << (8 * j), vc[u] |= cv << (8 * j);
+                }
+                if (kWhole || left > 0) {
+                    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + k) = mc[u];
+                    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + k) = vc[u];
+                    if (k % kGroup == 0) a.m_exp[k / kGroup] = (uint8_t)me[u], a.v_exp[k / kGroup] = (uint8_t)ve[u];
+                }
+            } else {
+                store_quad<float, kWhole>(static_cast<float*>(a.m) + k, left, m[u]);
+                store_quad<float, kWhole>(static_cast<float*>(a.v) + k, left, v[u]);
+            }
+            store_quad<P, kWhole>(param + i, left, w[u]);
+            if (master) store_quad<float, kWhole>(a.master + k, left, w[u]);
+        }
+    }
 }
 
 template <typename P, typename G, bool kBytes>
@@ -218,52 +383,9 @@ __global__ void __launch_bounds__(kBlock) k_adamw(const StepArgs a) {
         const G* grad = static_cast<const G*>(a.grads[which].data);
         if (!e.data || !grad) continue;
         const int64_t from = (tile - e.first_tile) * kTile;
-        const int64_t to = from + kTile < e.count ? from + kTile : e.count;
-        P* param = static_cast<P*>(e.data);
-        for (int64_t i0 = from; i0 < to; i0 += kBlock) {
-            const int64_t i = i0 + threadIdx.x, k = e.state_at + i;
-            const bool live = i < to;
-            float m = 0.0f, v = 0.0f, root = 0.0f;
-            uint8_t mb = 0, vb = 0;
-            if (kBytes) { /* the 32 lanes of a block share their exponents; those behind the tensor's end count as zero */
-                if (live) {
-                    mb = a.m_exp[k / kGroup], vb = a.v_exp[k / kGroup];
-                    m = code_value(static_cast<const uint8_t*>(a.m)[k]) * exponent_value(mb);
-                    const float u = code_value(static_cast<const uint8_t*>(a.v)[k]) * exponent_value(vb);
-                    v = u * u;
-                }
-            } else if (live) {
-                m = static_cast<const float*>(a.m)[k], v = static_cast<const float*>(a.v)[k];
-            }
-            if (live) {
-                const float g = to_float(grad[i]) * c.scale;
-                const float w = adamw(a.master ? a.master[k] : to_float(param[i]), m, v, root, g, a, c);
-                put(param + i, w);
-                if (a.master) a.master[k] = w;
-            }
-            if (kBytes) {
-                float most_m = fabsf(m), most_u = root;
-                for (int off = 16; off > 0; off >>= 1) { /* NaN wins: compared as bits */
-                    const uint32_t om = __float_as_uint(__shfl_xor(most_m, off, 64)), ou = __float_as_uint(__shfl_xor(most_u, off, 64));
-                    most_m = __uint_as_float(max(__float_as_uint(most_m), om));
-                    most_u = __uint_as_float(max(__float_as_uint(most_u), ou));
-                }
-                mb = block_exponent(most_m), vb = block_exponent(most_u);
-                if (live) {
-                    const uint32_t r = mix((uint32_t)k * 0x9E3779B1u + c.key);
-                    const float rm = (float)(r >> 16) * 0x1p-16f, rv = (float)(r & 0xffffu) * 0x1p-16f;
-                    const float sm = __uint_as_float((254u - mb) << 23), sv = __uint_as_float((254u - vb) << 23);
-                    const uint8_t cm = mb == 255 ? 0x7f : to_code(m * sm, rm);
-                    uint8_t cv = vb == 255 ? 0x7f : to_code(root * sv, rv);
-                    if (cv == 0 && root > 0.0f) cv = 1;
-                    static_cast<uint8_t*>(a.m)[k] = cm;
-                    static_cast<uint8_t*>(a.v)[k] = cv;
-                    if (k % kGroup == 0) a.m_exp[k / kGroup] = mb, a.v_exp[k / kGroup] = vb;
-                }
-            } else if (live) {
-                static_cast<float*>(a.m)[k] = m, static_cast<float*>(a.v)[k] = v;
-            }
-        }
+        P* param = static_cast<P*>(e.data) + from;
+        if (e.count - from >= kTile) step_tile<P, G, kBytes, true>(a, c, param, grad + from, e.state_at + from, kTile);
+        else step_tile<P, G, kBytes, false>(a, c, param, grad + from, e.state_at + from, (int)(e.count - from));
     }
 }
 

@@ -154,6 +154,9 @@ class AdamW:
         self._pointers = [p.data_ptr() for p in params]
         self._params_table = _Table(dev, self._pointers, self.counts)
         a = self._args = _lib.AdamWArgs()
+        size = _lib.load().mzs_grad_norm_workspace(self._params_table.tiles)
+        self._workspace = torch.empty(size, dtype=torch.uint8, device=dev)      # as the states, for one step at a time
+        a.workspace, a.workspace_bytes = self._workspace.data_ptr(), size
         a.device, a.n, a.param_dtype, a.state_bits = dev.index, len(params), _DTYPES[params[0].dtype], state_bits
         a.beta1, a.beta2, a.eps, a.weight_decay = self.betas[0], self.betas[1], eps, weight_decay
         a.exp_avg = self._state["exp_avg"].data_ptr()
@@ -255,7 +258,6 @@ class AdamW:
         else:
             a.lr_dev, a.lr = None, float(lr)
         a.max_norm, a.norm_given, a.norm_dev = float(self.max_grad_norm or 0.0), 0, self.grad_norm.data_ptr()
-        workspace = None
         if norm is not None:
             if self.max_grad_norm is None:
                 raise ValueError("norm: this optimizer has no max_grad_norm")
@@ -263,9 +265,5 @@ class AdamW:
                 raise ValueError("norm: one float32 value on the parameters' device")
             self.grad_norm.copy_(norm.reshape(()))
             a.norm_given = 1
-        elif self.max_grad_norm is not None:
-            size = _lib.load().mzs_grad_norm_workspace(a.n_tiles)
-            workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), size
         _lib.check(_lib.load().mzs_adamw_step(C.byref(a), stream.cuda_stream), "mzs_adamw_step")
         torch.autograd.graph.increment_version(self.params)
