@@ -428,7 +428,7 @@ typedef struct mzs_policy_args {
     int32_t device;             /* HIP device of every pointer below                                  */
     int32_t dtype;              /* MZS_DTYPE_* of logits and grad_logits                              */
     int64_t rows;
-    int64_t n_actions;          /* 1 .. 2^31 - 1                                                      */
+    int64_t n_actions;          /* 1 .. 2^28                                                          */
     const void* logits;         /* [rows][n_actions], a row every logits_stride elements (0: one row for all) */
     int64_t logits_stride;
     const uint8_t* mask;        /* 1 = allowed; a row every mask_stride bytes (0: one mask for all rows); NULL: all allowed */

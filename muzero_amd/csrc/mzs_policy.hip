@@ -17,7 +17,7 @@ namespace {
 
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr double kLog2e = 1.44269504088896340736;
-constexpr float kLow = -1e30f; /* stands for -inf where it is multiplied by an exponential that is 0 */
+constexpr float kLow = -1000.0f; /* exponents of 2 end here: 2^-1000 is 0, and 0 times a finite number stays 0 */
 
 struct Row {
     const void* logits;
@@ -33,38 +33,122 @@ struct Row {
     float c;     /* inverse_temperature * log2 e     */
 };
 
+typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+typedef w4 w4_any __attribute__((aligned(2))); /* rows may start at any element */
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+
+/* A logit type: kPer elements in 16 bytes.  get / set work on 16 bytes in registers, element j by a constant index. */
 template <typename T>
-__device__ __forceinline__ float to_float(T v);
+struct Kind;
 template <>
-__device__ __forceinline__ float to_float<float>(float v) {
-    return v;
-}
-struct bf16 {
-    uint16_t bits;
+struct Kind<float> {
+    static constexpr int kPer = 4;
+    static constexpr uint32_t kNone = 0xff800000u; /* -inf */
+    static __device__ __forceinline__ float load(const float* p) { return *p; }
+    static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
+    static __device__ __forceinline__ float get(const w4& v, int j) { return __uint_as_float(v[j]); }
+    static __device__ __forceinline__ void set(w4& v, int j, float x) { v[j] = __float_as_uint(x); }
+    static __device__ __forceinline__ void keep(w4& v, int j, bool k) { v[j] = k ? v[j] : kNone; }
+    static __device__ __forceinline__ w4 pack(const float* x) {
+        return w4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+    }
+};
+template <typename T>
+struct Half { /* two to a word */
+    static constexpr int kPer = 8;
+    static __device__ __forceinline__ void set_bits(w4& v, int j, uint32_t x) {
+        v[j >> 1] = j & 1 ? (v[j >> 1] & 0xffffu) | (x << 16) : (v[j >> 1] & 0xffff0000u) | x;
+    }
 };
 template <>
-__device__ __forceinline__ float to_float<bf16>(bf16 v) {
-    return __uint_as_float((uint32_t)v.bits << 16);
-}
+struct Kind<__bf16> : Half<__bf16> {
+    static constexpr uint32_t kNone = 0xff80u;
+    static __device__ __forceinline__ float load(const __bf16* p) {
+        return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16);
+    }
+    static __device__ __forceinline__ void store(__bf16* p, float v) { *p = (__bf16)v; }
+    static __device__ __forceinline__ float get(const w4& v, int j) {
+        return __uint_as_float(j & 1 ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16);
+    }
+    static __device__ __forceinline__ void keep(w4& v, int j, bool k) { if (!k) set_bits(v, j, kNone); }
+    static __device__ __forceinline__ w4 pack(const float* x) { /* v_cvt_pk_bf16_f32: nearest even, NaN kept */
+        w4 v;
+        _Pragma("unroll") for (int i = 0; i < 4; ++i)
+            v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x[2 * i], x[2 * i + 1]}), b2));
+        return v;
+    }
+};
 template <>
-__device__ __forceinline__ float to_float<_Float16>(_Float16 v) {
-    return (float)v;
+struct Kind<_Float16> : Half<_Float16> {
+    static constexpr uint32_t kNone = 0xfc00u;
+    static __device__ __forceinline__ float load(const _Float16* p) { return (float)*p; }
+    static __device__ __forceinline__ void store(_Float16* p, float v) { *p = (_Float16)v; }
+    static __device__ __forceinline__ float get(const w4& v, int j) {
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)(j & 1 ? v[j >> 1] >> 16 : v[j >> 1]));
+    }
+    static __device__ __forceinline__ void keep(w4& v, int j, bool k) { if (!k) set_bits(v, j, kNone); }
+    static __device__ __forceinline__ w4 pack(const float* x) {
+        w4 v;
+        _Pragma("unroll") for (int i = 0; i < 4; ++i)
+            v[i] = __builtin_bit_cast(uint32_t, h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
+        return v;
+    }
+};
+
+/* x moved `by` elements down, -inf behind them (by >= kPer: nothing is left) */
+template <typename T>
+__device__ __forceinline__ w4 move_down(const w4& x, uint32_t by) {
+    constexpr int kBits = 8 * sizeof(T);
+    const uint64_t none = (kBits == 32 ? Kind<T>::kNone : Kind<T>::kNone * 0x10001u) * 0x100000001ull;
+    const uint32_t bits = by < (uint32_t)Kind<T>::kPer ? by * kBits : 128u, sh = bits & 63u;
+    const uint64_t lo = x[0] | ((uint64_t)x[1] << 32), hi = x[2] | ((uint64_t)x[3] << 32);
+    const uint64_t a = bits == 128u ? none : bits & 64u ? hi : lo, b = bits >= 64u ? none : hi;
+    const uint64_t y0 = sh ? (a >> sh) | (b << (64u - sh)) : a, y1 = sh ? (b >> sh) | (none << (64u - sh)) : b;
+    return w4{(uint32_t)y0, (uint32_t)(y0 >> 32), (uint32_t)y1, (uint32_t)(y1 >> 32)};
+}
+
+/* N vectors of a row from element i on, `stride` elements apart; what the mask forbids and what lies behind the row's end is -inf.  Every
+ * lane loads inside the row (n >= kPer): a vector that the end cuts is loaded from n - kPer on and moved down, so that the
+ * loads go out back to back whatever the row's end.  l and mask are uniform over the block: scalar base, 32-bit byte offset. */
+template <typename T, int N>
+__device__ __forceinline__ void load_vecs(const T* __restrict__ l, const uint8_t* __restrict__ mask, uint32_t i, uint32_t stride, uint32_t n,
+                                          w4* x) {
+    constexpr int kPer = Kind<T>::kPer;
+    uint32_t at[N];
+    _Pragma("unroll") for (int u = 0; u < N; ++u) {
+        at[u] = min(i + u * stride, n - kPer);
+        x[u] = *reinterpret_cast<const w4_any*>(reinterpret_cast<const char*>(l) + (uint32_t)(at[u] * sizeof(T)));
+    }
+    if (mask) {
+        uint32_t m[N][kPer / 4];
+        _Pragma("unroll") for (int u = 0; u < N; ++u) __builtin_memcpy(m[u], mask + at[u], kPer);
+        _Pragma("unroll") for (int u = 0; u < N; ++u)
+            _Pragma("unroll") for (int j = 0; j < kPer; ++j) Kind<T>::keep(x[u], j, (m[u][j / 4] >> (8 * (j % 4))) & 0xffu);
+    }
+    _Pragma("unroll") for (int u = 0; u < N; ++u)
+        if (i + u * stride > n - kPer) x[u] = move_down<T>(x[u], i + u * stride - at[u]);
 }
 template <typename T>
-__device__ __forceinline__ T from_float(float v);
-template <>
-__device__ __forceinline__ float from_float<float>(float v) {
-    return v;
+__device__ __forceinline__ w4 load_vec(const T* __restrict__ l, const uint8_t* __restrict__ mask, uint32_t i, uint32_t n) {
+    w4 x;
+    load_vecs<T, 1>(l, mask, i, 0, n, &x);
+    return x;
 }
-template <>
-__device__ __forceinline__ bf16 from_float<bf16>(float v) { /* round to nearest even; a NaN stays one */
-    uint32_t b = __float_as_uint(v);
-    b = v != v ? 0x7fc00000u : b + 0x7fffu + ((b >> 16) & 1u);
-    return bf16{(uint16_t)(b >> 16)};
-}
-template <>
-__device__ __forceinline__ _Float16 from_float<_Float16>(float v) {
-    return (_Float16)v;
+/* the elements of v that the row has go to [i, i + kPer) */
+template <typename T>
+__device__ __forceinline__ void store_vec(T* __restrict__ g, uint32_t i, uint32_t n, const w4& v) {
+    constexpr int kPer = Kind<T>::kPer;
+    if (i + kPer <= n) {
+        *reinterpret_cast<w4_any*>(reinterpret_cast<char*>(g) + (uint32_t)(i * sizeof(T))) = v;
+    } else if (i < n) { /* one thread's: short code before fast code */
+        const uint64_t w0 = v[0] | ((uint64_t)v[1] << 32), w1 = v[2] | ((uint64_t)v[3] << 32);
+        _Pragma("clang loop unroll(disable)") for (uint32_t j = 0; i + j < n; ++j) {
+            const uint32_t bit = j * 8 * sizeof(T), bits = (uint32_t)((bit < 64u ? w0 : w1) >> (bit & 63u));
+            __builtin_memcpy(g + i + j, &bits, sizeof(T));
+        }
+    }
 }
 
 /* one part of a row: its largest logit, and s and t relative to it */
@@ -97,108 +181,555 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 
 constexpr int kBlock = 256;
+constexpr float kInf = __builtin_inff();
 
-__device__ __forceinline__ void write_row(const Row& p, int64_t r, Sum v, float l_action, int64_t a) {
-    const bool empty = v.s == 0.0f;
-    const float log2_s = log2f(v.s), log_total = kLn2 * log2_s;
-    p.log_z[r] = empty ? -__builtin_inff() : p.scale * v.big + log_total;
-    p.entropy[r] = empty ? 0.0f : kLn2 * (log2_s - v.t / v.s);
+/* Butterfly over G consecutive lanes: every lane gets the same bits (at each step both partners combine the same two values). */
+template <int G, typename F>
+__device__ __forceinline__ float lanes_reduce(float v, F op) {
+    if (G > 1) v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true)));   /* lane ^ 1 */
+    if (G > 2) v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true)));   /* lane ^ 2 */
+    if (G > 4) v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xf, 0xf, true)));  /* the other four of eight */
+    if (G > 8) v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xf, 0xf, true)));  /* the other eight of 16 */
+    if (G > 16) v = op(v, __shfl_xor(v, 16, 64));
+    if (G > 32) v = op(v, __shfl_xor(v, 32, 64));
+    return v;
+}
+template <int G>
+__device__ __forceinline__ float lanes_max(float v) {
+    return lanes_reduce<G>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
+    return lanes_reduce<G>(v, [](float a, float b) { return a + b; });
+}
+
+/* exponent of 2 for a logit x beside the row's largest one; finite, so that 0 * it is 0 */
+__device__ __forceinline__ float exponent_of(const Row& p, float x, float big) { return fmaxf(p.c * (x - big), kLow); }
+/* 2^d; a NaN logit (which fmaxf turned into kLow) stays one */
+__device__ __forceinline__ float power_of(float d, float x) { return x != x ? x : __builtin_amdgcn_exp2f(d); }
+
+struct Values {
+    float log_z, entropy, log_total, log2_s;
+    bool empty;
+};
+__device__ __forceinline__ Values row_values(const Row& p, const Sum& v) {
+    Values o;
+    o.empty = v.s == 0.0f;
+    o.log2_s = log2f(v.s);
+    o.log_total = kLn2 * o.log2_s;
+    o.log_z = o.empty ? -kInf : p.scale * v.big + o.log_total;
+    o.entropy = o.empty ? 0.0f : kLn2 * (o.log2_s - v.t / v.s);
+    return o;
+}
+__device__ __forceinline__ void write_row(const Row& p, int64_t r, const Sum& v, const Values& o, float l_action, int64_t a) {
+    p.log_z[r] = o.log_z;
+    p.entropy[r] = o.entropy;
     p.row_stats[2 * r] = v.big;
     p.row_stats[2 * r + 1] = v.s;
     float lp = 0.0f;
     if (a >= p.n) lp = __builtin_nanf("");
-    else if (a >= 0) lp = empty ? -__builtin_inff() : p.scale * (l_action - v.big) - log_total;
+    else if (a >= 0) lp = o.empty ? -kInf : p.scale * (l_action - v.big) - o.log_total;
     p.log_prob[r] = lp;
 }
-
-/* One block per row, one logit a thread and step. */
 template <typename T>
-__global__ void __launch_bounds__(kBlock) k_policy_rows(const Row p) {
-    __shared__ Sum parts[kBlock];
-    __shared__ uint64_t keys[kBlock];
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+__device__ __forceinline__ float action_logit(const Row& p, const T* l, const uint8_t* mask, int64_t a) {
+    return a < 0 || a >= p.n ? 0.0f : mask && !mask[a] ? -kInf : Kind<T>::load(l + a);
+}
+__device__ __forceinline__ void write_top(const Row& p, int64_t r, int k, uint64_t key, const Sum& v, const Values& o) {
+    p.top_action[r * p.top + k] = key ? (int32_t)(0xffffffffu - (uint32_t)key) : -1;
+    p.top_log_prob[r * p.top + k] = key ? p.scale * (key_value(key) - v.big) - o.log_total : -kInf;
+}
+
+/* What the gradient of a row needs: grad_i = e_i (base + slope d_i), + at_action where i is the action. */
+struct Slope {
+    float big, base, slope, at_action;
+    bool empty;
+};
+__device__ __forceinline__ Slope row_slope(const Row& p, int64_t r, int64_t a, const Sum& v, float entropy, float log2_s) {
+    const float ga = a < 0 || !p.grad_log_prob ? 0.0f : a >= p.n ? __builtin_nanf("") : p.grad_log_prob[r];
+    const float gh = p.grad_entropy ? p.grad_entropy[r] : 0.0f, gz = p.grad_log_z ? p.grad_log_z[r] : 0.0f;
+    const float f = p.scale / v.s; /* log p_i = ln 2 (d_i - log2 s) */
+    Slope q;
+    q.big = v.big;
+    q.base = f * (gz - ga - gh * (entropy - kLn2 * log2_s));
+    q.slope = f * (-gh * kLn2);
+    q.at_action = p.scale * ga;
+    q.empty = v.s == 0.0f;
+    return q;
+}
+__device__ __forceinline__ float slope_at(const Row& p, const Slope& q, float x) {
+    const float d = exponent_of(p, x, q.big);
+    return power_of(d, x) * (q.base + q.slope * d);
+}
+
+/* ------------------------------------------------------------------ narrow rows
+ * G lanes hold a row of up to G * E logits in registers, 64 / G rows to a wave: one read, one write, no shared memory.  The choice of
+ * G and E by n is in launch_lanes. */
+template <typename T, int G, int E, bool kForward, bool kGrad>
+__global__ void __launch_bounds__(kBlock) k_policy_lanes(const Row p) {
+    constexpr int kRows = kBlock / G;
+    const int g = threadIdx.x % G;
+    const int n = (int)p.n;
+    for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < p.rows; r0 += (int64_t)gridDim.x * kRows) {
+        const int64_t r_mine = r0 + threadIdx.x / G;
+        const bool live = r_mine < p.rows;
+        const int64_t r = live ? r_mine : p.rows - 1; /* lanes without a row shadow the last one: every lane takes part in the butterflies */
         const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
         const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
-        Sum v{-__builtin_inff(), 0.0f, 0.0f};
-        for (int64_t i = threadIdx.x; i < p.n; i += kBlock) {
-            if (mask && !mask[i]) continue;
-            const float x = to_float(l[i]);
-            if (x == -__builtin_inff()) continue;
-            v = sum_merge(v, Sum{x != x ? v.big : x, x != x ? x : 1.0f, 0.0f}, p.c);
+        const int64_t a = row_action(p, r);
+        float x[E];
+        _Pragma("unroll") for (int j = 0; j < E; ++j) {
+            const int i = g + j * G;
+            x[j] = i < n ? Kind<T>::load(l + i) : -kInf;
         }
-        parts[threadIdx.x] = v;
-        __syncthreads();
-        for (int w = kBlock / 2; w > 0; w >>= 1) {
-            if (threadIdx.x < (unsigned)w) parts[threadIdx.x] = sum_merge(parts[threadIdx.x], parts[threadIdx.x + w], p.c);
+        if (mask) {
+            _Pragma("unroll") for (int j = 0; j < E; ++j) {
+                const int i = g + j * G;
+                if (i < n && !mask[i]) x[j] = -kInf;
+            }
+        }
+        const float la = kForward ? action_logit<T>(p, l, mask, a) : 0.0f;
+        Sum v{-kInf, 0.0f, 0.0f};
+        _Pragma("unroll") for (int j = 0; j < E; ++j) v.big = fmaxf(v.big, x[j]);
+        v.big = lanes_max<G>(v.big);
+        if (v.big > -kInf) {
+            _Pragma("unroll") for (int j = 0; j < E; ++j) {
+                const float d = exponent_of(p, x[j], v.big), e = power_of(d, x[j]);
+                v.s += e, v.t = fmaf(e, d, v.t);
+            }
+        } else { /* nothing allowed, or nothing but NaN */
+            _Pragma("unroll") for (int j = 0; j < E; ++j) if (x[j] != x[j]) v.s = x[j];
+        }
+        v.s = lanes_sum<G>(v.s), v.t = lanes_sum<G>(v.t);
+        if (v.big == kInf) v.s = __builtin_nanf("");
+        const Values o = row_values(p, v);
+        if (kForward && live && g == 0) write_row(p, r, v, o, la, a);
+        if (kForward && p.top > 0) {
+            uint32_t key[E];
+            _Pragma("unroll") for (int j = 0; j < E; ++j)
+                key[j] = x[j] == -kInf ? 0u : (uint32_t)(rank_key(x[j], 0) >> 32);
+            uint64_t last = ~0ull;
+            for (int k = 0; k < p.top; ++k) {
+                uint64_t best = 0;
+                _Pragma("unroll") for (int j = 0; j < E; ++j) {
+                    const uint64_t c = key[j] ? ((uint64_t)key[j] << 32) | (0xffffffffu - (uint32_t)(g + j * G)) : 0;
+                    if (c < last && c > best) best = c;
+                }
+                _Pragma("unroll") for (int off = 1; off < G; off <<= 1) {
+                    const uint64_t other = __shfl_xor((unsigned long long)best, off, 64);
+                    best = other > best ? other : best;
+                }
+                last = best;
+                if (live && g == 0) write_top(p, r, k, last, v, o);
+            }
+        }
+        if (kGrad) {
+            const Slope q = row_slope(p, r, a, v, o.entropy, o.log2_s);
+            T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
+            _Pragma("unroll") for (int j = 0; j < E; ++j) {
+                const int i = g + j * G;
+                float y = 0.0f;
+                if (!q.empty && x[j] != -kInf) {
+                    y = slope_at(p, q, x[j]);
+                    if (i == a) y += q.at_action;
+                }
+                if (live && i < n) Kind<T>::store(out + i, y);
+            }
+        }
+    }
+}
+
+/* ------------------------------------------------------------------ wide rows
+ * A block walks a chunk of a row: thread t takes the 16-byte vectors t, t + kBlock, ... of it. */
+
+/* merges every thread's part; all threads return the whole.  lds: 3 floats a wave */
+template <int kThreads>
+__device__ __forceinline__ Sum block_merge(const Row& p, Sum v, float* lds) {
+    constexpr int kWaves = kThreads / 64;
+    const int wave = threadIdx.x >> 6;
+    float big = lanes_max<64>(v.big);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[wave] = big;
+    __syncthreads();
+    _Pragma("unroll") for (int w = 0; w < kWaves; ++w) big = fmaxf(big, lds[w]);
+    const float d = v.big == big ? 0.0f : fmaxf(p.c * (v.big - big), kLow), f = __builtin_amdgcn_exp2f(d);
+    const float s = lanes_sum<64>(f * v.s), t = lanes_sum<64>(f * (v.t + d * v.s));
+    if ((threadIdx.x & 63) == 0) lds[kWaves + wave] = s, lds[2 * kWaves + wave] = t;
+    __syncthreads();
+    Sum o{big, 0.0f, 0.0f};
+    _Pragma("unroll") for (int w = 0; w < kWaves; ++w) o.s += lds[kWaves + w], o.t += lds[2 * kWaves + w];
+    if (big == kInf) o.s = __builtin_nanf("");
+    return o;
+}
+
+constexpr int kAhead = 4; /* vectors a thread has in flight */
+
+/* The compiler may not look behind this: a row held packed is unpacked anew in each pass over it, a vector at a time, where it would
+ * otherwise keep every unpacked value (twice the registers, which spill). */
+__device__ __forceinline__ void unpack_here(w4& v) { asm volatile("" : "+v"(v)); }
+
+/* takes kPer * N logits into a thread's running sum: their maximum first, one rescaling, then the exponentials */
+template <typename T, int N>
+__device__ __forceinline__ void sum_vecs(const Row& p, w4* v, Sum& sum) {
+    constexpr int kPer = Kind<T>::kPer;
+    float big = sum.big;
+    _Pragma("unroll") for (int u = 0; u < N; ++u) {
+        if (N > kAhead) unpack_here(v[u]);
+        _Pragma("unroll") for (int j = 0; j < kPer; ++j) big = fmaxf(big, Kind<T>::get(v[u], j));
+    }
+    const float shift = sum.big == big ? 0.0f : fmaxf(p.c * (sum.big - big), kLow), f = __builtin_amdgcn_exp2f(shift);
+    float s = f * sum.s, t = f * (sum.t + shift * sum.s);
+    const float ref = big == -kInf ? 0.0f : big; /* nothing allowed so far: every exponential is 0 (or NaN) */
+    _Pragma("unroll") for (int u = 0; u < N; ++u) {
+        if (N > kAhead) unpack_here(v[u]);
+        _Pragma("unroll") for (int j = 0; j < kPer; ++j) {
+            const float x = Kind<T>::get(v[u], j);
+            const float d0 = p.c * (x - ref), e = __builtin_amdgcn_exp2f(d0);
+            s += e, t = fmaf(e, fmaxf(d0, kLow), t);
+        }
+    }
+    sum = Sum{big, s, t};
+}
+
+constexpr int kHistogram = 256;
+constexpr int kStrips = 512;  /* strips that can hold alternatives              */
+constexpr int kKeys = 1024;   /* logits that can be alternatives                */
+struct TopScratch {
+    uint32_t histogram[kHistogram];
+    uint32_t strips[kStrips];
+    uint64_t keys[kKeys];
+    uint32_t n_strips, n_keys, bin, rest;
+    uint64_t best[kBlock / 64 * 4];
+};
+
+__device__ __forceinline__ uint32_t rank_value(float x) { return x == -kInf ? 0u : (uint32_t)(rank_key(x, 0) >> 32); }
+
+/* A strip: the vectors that one thread took of one chunk, with the largest of their logits.  The `top` largest logits of a row lie at or
+ * above the top-th largest strip maximum tau (that many strips have one there), so:
+ *   1. tau from a radix selection over the strips' maxima, 8 bits of the ordered value a pass;
+ *   2. strips whose maximum reaches tau are read again, logits that reach it are collected;
+ *   3. a collected logit's rank is the number of collected ones before it.
+ * After two passes tau is known to 16 bits, which collects little more than it has to — unless many logits are alike.  Then the selection
+ * goes on to all 32 bits, logits above tau are collected (there are fewer than `top` strips of them), and the ones equal
+ * to tau are taken from the row's start on.  A row where even that is too much (or with NaN) is searched `top` times. */
+template <typename T, int kThreads, typename Maximum>
+__device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* mask, const Sum& v, const Values& o, Maximum maximum,
+                           int n_strips, int chunk_vecs, uint32_t chunk_len, TopScratch& sh) {
+    constexpr int kPer = Kind<T>::kPer;
+    const int tid = threadIdx.x;
+    const uint32_t want = (uint32_t)p.top;
+    const uint32_t n = (uint32_t)p.n;
+    uint32_t tau = 0, fixed = 0; /* the bits of tau known so far, and which */
+    bool done = false;
+    const bool plain = v.s == v.s;
+    for (int stage = 0; stage < 2 && plain && !done; ++stage) {
+        uint32_t left = want;
+        if (stage) { /* go on from the 16 bits: how many strips are above them */
+            if (tid == 0) sh.rest = 0;
+            __syncthreads();
+            uint32_t above = 0;
+            for (int i = tid; i < n_strips; i += kThreads) above += (rank_value(maximum(i)) & fixed) > tau;
+            if (above) atomicAdd(&sh.rest, above);
+            __syncthreads();
+            left = want > sh.rest ? want - sh.rest : 1u;
             __syncthreads();
         }
-        v = parts[0];
-        if (v.big == __builtin_inff()) v.s = __builtin_nanf("");
-        if (threadIdx.x == 0) {
-            const int64_t a = row_action(p, r);
-            const float la = a < 0 || a >= p.n ? 0.0f : mask && !mask[a] ? -__builtin_inff() : to_float(l[a]);
-            write_row(p, r, v, la, a);
+        for (int pass = 2 * stage; pass < 2 * stage + 2; ++pass) {
+            const int shift = 24 - 8 * pass;
+            for (int i = tid; i < kHistogram; i += kThreads) sh.histogram[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < n_strips; i += kThreads) {
+                const uint32_t k = rank_value(maximum(i));
+                if (k && (k & fixed) == tau) atomicAdd(&sh.histogram[(k >> shift) & 255u], 1u);
+            }
+            __syncthreads();
+            if (tid < 64) { /* lane i: bins 4 i .. 4 i + 3; counts from the top */
+                uint32_t c[4], mine = 0;
+                for (int j = 0; j < 4; ++j) mine += c[j] = sh.histogram[4 * tid + j];
+                uint32_t above = mine;
+                for (int off = 1; off < 64; off <<= 1) {
+                    const uint32_t other = __shfl_down(above, off, 64);
+                    if (tid + off < 64) above += other;
+                }
+                above -= mine; /* strips in the bins of higher lanes */
+                if (tid == 0) sh.bin = 0, sh.rest = left;
+                __builtin_amdgcn_wave_barrier();
+                if (above < left && above + mine >= left) {
+                    uint32_t higher = above;
+                    for (int j = 3; j >= 0; --j) {
+                        if (higher < left && higher + c[j] >= left) sh.bin = 4 * tid + j, sh.rest = left - higher;
+                        higher += c[j];
+                    }
+                }
+            }
+            __syncthreads();
+            tau |= sh.bin << shift, fixed |= 255u << shift;
+            left = sh.rest;
+            __syncthreads();
         }
-        uint64_t last = ~0ull;
-        for (int k = 0; k < p.top; ++k) {
-            uint64_t best = 0;
-            for (int64_t i = threadIdx.x; i < p.n; i += kBlock) {
-                if (mask && !mask[i]) continue;
-                const float x = to_float(l[i]);
-                const uint64_t key = x == -__builtin_inff() ? 0 : rank_key(x, (uint32_t)i);
+        /* strips and logits at or above tau (second stage: above) */
+        if (tid == 0) sh.n_strips = 0, sh.n_keys = 0;
+        __syncthreads();
+        const uint32_t least = stage ? tau + 1u : tau > 0u ? tau : 1u;
+        for (int i = tid; i < n_strips; i += kThreads)
+            if (rank_value(maximum(i)) >= least) {
+                const uint32_t at = atomicAdd(&sh.n_strips, 1u);
+                if (at < kStrips) sh.strips[at] = i;
+            }
+        __syncthreads();
+        const uint32_t found = sh.n_strips;
+        if (found <= kStrips) {
+            for (uint32_t w = tid; w < found * chunk_vecs; w += kThreads) {
+                const uint32_t strip = sh.strips[w / chunk_vecs], j = w % chunk_vecs;
+                const uint32_t chunk = strip / kThreads, t = strip % kThreads;
+                const uint32_t i = chunk * chunk_len + (j * kThreads + t) * kPer; /* below n rounded up to a chunk's vectors: 32 bits */
+                if (i >= n) continue;
+                const w4 x = load_vec<T>(l, mask, i, n);
+                _Pragma("unroll") for (int q = 0; q < kPer; ++q) {
+                    const uint32_t k = rank_value(Kind<T>::get(x, q));
+                    if (k >= least) {
+                        const uint32_t at = atomicAdd(&sh.n_keys, 1u);
+                        if (at < kKeys) sh.keys[at] = ((uint64_t)k << 32) | (0xffffffffu - (i + q));
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const uint32_t n_keys = sh.n_keys;
+        done = found <= kStrips && n_keys <= kKeys;
+        if (done) {
+            for (uint32_t i = tid; i < n_keys; i += kThreads) {
+                const uint64_t key = sh.keys[i];
+                uint32_t rank = 0;
+                for (uint32_t k = 0; k < n_keys; ++k) rank += sh.keys[k] > key;
+                if (rank < want) write_top(p, r, rank, key, v, o);
+            }
+            uint32_t at = n_keys < want ? n_keys : want;
+            if (stage && tau) { /* equal ones in the row's order */
+                for (uint32_t i0 = 0; i0 < n && at < want; i0 += kThreads * kPer) {
+                    const uint32_t i = i0 + tid * kPer;
+                    uint32_t hit = 0;
+                    if (i < n) {
+                        const w4 x = load_vec<T>(l, mask, i, n);
+                        _Pragma("unroll") for (int q = 0; q < kPer; ++q) hit |= (uint32_t)(rank_value(Kind<T>::get(x, q)) == tau) << q;
+                    }
+                    uint32_t before = __popc(hit);
+                    const uint32_t mine = before;
+                    for (int off = 1; off < 64; off <<= 1) {
+                        const uint32_t other = __shfl_up(before, off, 64);
+                        if ((tid & 63) >= off) before += other;
+                    }
+                    if ((tid & 63) == 63) sh.histogram[tid >> 6] = before;
+                    __syncthreads();
+                    uint32_t slot = at + before - mine, all = 0;
+                    for (int w = 0; w < kThreads / 64; ++w) {
+                        if (w < (tid >> 6)) slot += sh.histogram[w];
+                        all += sh.histogram[w];
+                    }
+                    for (int q = 0; q < kPer; ++q)
+                        if ((hit >> q) & 1u) {
+                            if (slot < want) write_top(p, r, slot, ((uint64_t)tau << 32) | (0xffffffffu - (uint32_t)(i + q)), v, o);
+                            ++slot;
+                        }
+                    at = at + all < want ? at + all : want;
+                    __syncthreads();
+                }
+            }
+            for (uint32_t k = at + tid; k < want; k += kThreads) write_top(p, r, k, 0, v, o);
+        }
+        __syncthreads();
+    }
+    if (done) return;
+    uint64_t last = ~0ull;
+    for (uint32_t k = 0; k < want; ++k) {
+        uint64_t best = 0;
+        for (uint32_t i = tid * kPer; i < n; i += kThreads * kPer) {
+            const w4 x = load_vec<T>(l, mask, i, n);
+            _Pragma("unroll") for (int q = 0; q < kPer; ++q) {
+                const uint32_t c = rank_value(Kind<T>::get(x, q));
+                const uint64_t key = c ? ((uint64_t)c << 32) | (0xffffffffu - (uint32_t)(i + q)) : 0;
                 if (key < last && key > best) best = key;
             }
-            keys[threadIdx.x] = best;
-            __syncthreads();
-            for (int w = kBlock / 2; w > 0; w >>= 1) {
-                if (threadIdx.x < (unsigned)w && keys[threadIdx.x + w] > keys[threadIdx.x])
-                    keys[threadIdx.x] = keys[threadIdx.x + w];
-                __syncthreads();
-            }
-            last = keys[0];
-            if (threadIdx.x == 0) {
-                const float log_total = kLn2 * log2f(v.s);
-                p.top_action[r * p.top + k] = last ? (int32_t)(0xffffffffu - (uint32_t)last) : -1;
-                p.top_log_prob[r * p.top + k] =
-                    last ? p.scale * (key_value(last) - v.big) - log_total : -__builtin_inff();
-            }
-            __syncthreads();
         }
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint64_t other = __shfl_xor((unsigned long long)best, off, 64);
+            best = other > best ? other : best;
+        }
+        if ((tid & 63) == 0) sh.best[tid >> 6] = best;
+        __syncthreads();
+        for (int w = 0; w < kThreads / 64; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+        last = best;
+        if (tid == 0) write_top(p, r, k, last, v, o);
         __syncthreads();
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kBlock) k_policy_grad(const Row p) {
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
-        const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
-        T* g = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
-        const int64_t a = row_action(p, r);
-        const float big = p.row_stats[2 * r], s = p.row_stats[2 * r + 1];
-        const bool empty = s == 0.0f;
-        const float log2_s = log2f(s);
-        const float ga = a < 0 || !p.grad_log_prob ? 0.0f : a >= p.n ? __builtin_nanf("") : p.grad_log_prob[r];
-        const float gh = p.grad_entropy ? p.grad_entropy[r] : 0.0f, gz = p.grad_log_z ? p.grad_log_z[r] : 0.0f;
-        const float base = gz - ga - gh * p.entropy[r];
-        for (int64_t i = threadIdx.x; i < p.n; i += kBlock) {
-            const float x = to_float(l[i]);
-            float out = 0.0f;
-            if (!empty && !(mask && !mask[i]) && x != -__builtin_inff()) {
-                const float d = fmaxf(p.c * (x - big), kLow), e = x != x ? x : __builtin_amdgcn_exp2f(d);
-                out = e / s * (base - gh * (kLn2 * (d - log2_s)));
-                if (i == a) out += ga;
-                out *= p.scale;
-            }
-            g[i] = from_float<T>(out);
+/* kSplit: the chunk's part goes to parts[row][chunk] and its strips' maxima to strips[row][chunk][thread]; else the chunk is the row */
+template <typename T, bool kSplit>
+__global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks, int chunk_vecs, float* __restrict__ parts,
+                                                         float* __restrict__ strips) {
+    constexpr int kPer = Kind<T>::kPer;
+    __shared__ float lds[3 * (kBlock / 64)];
+    const int64_t r = blockIdx.x / chunks;
+    const int chunk = blockIdx.x % chunks;
+    const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
+    const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
+    const uint32_t n = (uint32_t)p.n;
+    const uint32_t chunk_len = (uint32_t)chunk_vecs * kBlock * kPer, from = chunk * chunk_len + threadIdx.x * kPer;
+    Sum v{-kInf, 0.0f, 0.0f};
+    int j = 0;
+    for (; j + kAhead <= chunk_vecs; j += kAhead) {
+        w4 x[kAhead];
+        load_vecs<T, kAhead>(l, mask, from + (uint32_t)j * kBlock * kPer, kBlock * kPer, n, x);
+        sum_vecs<T, kAhead>(p, x, v);
+    }
+    for (; j < chunk_vecs; ++j) {
+        w4 x = load_vec<T>(l, mask, from + (uint32_t)j * kBlock * kPer, n);
+        sum_vecs<T, 1>(p, &x, v);
+    }
+    const float mine = v.big;
+    v = block_merge<kBlock>(p, v, lds);
+    if constexpr (kSplit) {
+        if (p.top > 0) strips[(int64_t)blockIdx.x * kBlock + threadIdx.x] = mine;
+        if (threadIdx.x == 0) {
+            float* q = parts + 3 * (int64_t)blockIdx.x;
+            q[0] = v.big, q[1] = v.s, q[2] = v.t;
         }
+    } else {
+        __shared__ float maxima[kBlock];
+        __shared__ TopScratch top;
+        const Values o = row_values(p, v);
+        if (threadIdx.x == 0) {
+            const int64_t a = row_action(p, r);
+            write_row(p, r, v, o, action_logit<T>(p, l, mask, a), a);
+        }
+        if (p.top > 0) {
+            maxima[threadIdx.x] = mine;
+            __syncthreads();
+            select_top<T, kBlock>(p, r, l, mask, v, o, [&](int i) { return maxima[i]; }, kBlock, chunk_vecs, chunk_len, top);
+        }
+    }
+}
+
+/* joins the parts of each row's chunks (at most kBlock of them) */
+template <typename T>
+__global__ void __launch_bounds__(kBlock) k_policy_join(const Row p, int chunks, int chunk_vecs, const float* __restrict__ parts,
+                                                        const float* __restrict__ strips) {
+    __shared__ float lds[3 * (kBlock / 64)];
+    __shared__ TopScratch top;
+    const int64_t r = blockIdx.x;
+    const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
+    const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
+    Sum v{-kInf, 0.0f, 0.0f};
+    if ((int)threadIdx.x < chunks) {
+        const float* q = parts + 3 * (r * chunks + threadIdx.x);
+        v = Sum{q[0], q[1], q[2]};
+    }
+    v = block_merge<kBlock>(p, v, lds);
+    const Values o = row_values(p, v);
+    if (threadIdx.x == 0) {
+        const int64_t a = row_action(p, r);
+        write_row(p, r, v, o, action_logit<T>(p, l, mask, a), a);
+    }
+    if (p.top > 0) {
+        const float* mine = strips + r * chunks * kBlock;
+        select_top<T, kBlock>(p, r, l, mask, v, o, [&](int i) { return mine[i]; }, chunks * kBlock, chunk_vecs,
+                              (uint32_t)chunk_vecs * kBlock * Kind<T>::kPer, top);
+    }
+}
+
+/* gradient of one vector */
+template <typename T>
+__device__ __forceinline__ w4 slope_vec(const Row& p, const Slope& q, const w4& x, uint32_t i, uint32_t action) {
+    constexpr int kPer = Kind<T>::kPer;
+    float y[kPer];
+    _Pragma("unroll") for (int j = 0; j < kPer; ++j) {
+        const float l = Kind<T>::get(x, j);
+        const float d0 = p.c * (l - q.big), e = __builtin_amdgcn_exp2f(d0);
+        y[j] = e * fmaf(q.slope, fmaxf(d0, kLow), q.base);
+    }
+    if (action - i < kPer)
+        _Pragma("unroll") for (int j = 0; j < kPer; ++j) if (i + j == action && Kind<T>::get(x, j) != -kInf) y[j] += q.at_action;
+    if (!(fabsf(q.base) < kInf)) /* NaN or infinite coefficients: elements that are not allowed stay 0 all the same */
+        _Pragma("unroll") for (int j = 0; j < kPer; ++j) if (Kind<T>::get(x, j) == -kInf) y[j] = 0.0f;
+    return Kind<T>::pack(y);
+}
+
+/* gradient of chunks from the rows' stored statistics */
+template <typename T>
+__global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks, int chunk_vecs) {
+    constexpr int kPer = Kind<T>::kPer;
+    const int64_t r = blockIdx.x / chunks;
+    const int chunk = blockIdx.x % chunks;
+    const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
+    const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
+    T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
+    const int64_t a = row_action(p, r);
+    const Sum v{p.row_stats[2 * r], p.row_stats[2 * r + 1], 0.0f};
+    const Slope q = row_slope(p, r, a, v, p.entropy[r], log2f(v.s));
+    const uint32_t n = (uint32_t)p.n, action = a >= 0 && a < p.n ? (uint32_t)a : ~0u;
+    const uint32_t from = ((uint32_t)chunk * chunk_vecs * kBlock + threadIdx.x) * kPer;
+    int j = 0;
+    for (; j + kAhead <= chunk_vecs; j += kAhead) {
+        w4 x[kAhead];
+        const uint32_t i = from + (uint32_t)j * kBlock * kPer;
+        load_vecs<T, kAhead>(l, mask, i, kBlock * kPer, n, x);
+        _Pragma("unroll") for (int u = 0; u < kAhead; ++u) {
+            const uint32_t at = i + u * kBlock * kPer;
+            store_vec<T>(out, at, n, q.empty ? w4{0, 0, 0, 0} : slope_vec<T>(p, q, x[u], at, action));
+        }
+    }
+    for (; j < chunk_vecs; ++j) {
+        const uint32_t i = from + (uint32_t)j * kBlock * kPer;
+        const w4 x = load_vec<T>(l, mask, i, n);
+        store_vec<T>(out, i, n, q.empty ? w4{0, 0, 0, 0} : slope_vec<T>(p, q, x, i, action));
+    }
+}
+
+/* Forward and gradient of a row that a block holds in registers (V 16-byte vectors a thread): one read and one write of memory. */
+template <typename T, int kThreads, int V>
+__global__ void __launch_bounds__(kThreads) k_policy_train(const Row p) {
+    constexpr int kPer = Kind<T>::kPer;
+    __shared__ float lds[3 * (kThreads / 64)];
+    __shared__ float maxima[kThreads];
+    __shared__ TopScratch top;
+    const int64_t r = blockIdx.x;
+    const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
+    const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
+    const uint32_t n = (uint32_t)p.n, from = threadIdx.x * kPer;
+    w4 x[V];
+    constexpr int kGroup = V < kAhead ? V : kAhead;
+    static_assert(V % kGroup == 0, "whole groups");
+    _Pragma("unroll") for (int j = 0; j < V; j += kGroup)
+        load_vecs<T, kGroup>(l, mask, from + j * kThreads * kPer, kThreads * kPer, n, x + j);
+    const int64_t a = row_action(p, r);
+    const float la = action_logit<T>(p, l, mask, a); /* before the gradient may overwrite it */
+    Sum v{-kInf, 0.0f, 0.0f};
+    sum_vecs<T, V>(p, x, v);
+    const float mine = v.big;
+    v = block_merge<kThreads>(p, v, lds);
+    const Values o = row_values(p, v);
+    if (threadIdx.x == 0) write_row(p, r, v, o, la, a);
+    if (p.top > 0) {
+        maxima[threadIdx.x] = mine;
+        __syncthreads();
+        select_top<T, kThreads>(p, r, l, mask, v, o, [&](int i) { return maxima[i]; }, kThreads, V, (uint32_t)V * kThreads * kPer, top);
+        __syncthreads();
+    }
+    const Slope q = row_slope(p, r, a, v, o.entropy, o.log2_s);
+    T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
+    const uint32_t action = a >= 0 && a < p.n ? (uint32_t)a : ~0u;
+    _Pragma("unroll") for (int j = 0; j < V; ++j) {
+        const uint32_t i = from + j * kThreads * kPer;
+        if (V > kAhead) unpack_here(x[j]);
+        store_vec<T>(out, i, n, q.empty ? w4{0, 0, 0, 0} : slope_vec<T>(p, q, x[j], i, action));
     }
 }
 
 int check(const mzs_policy_args* a, bool forward, bool grad) {
     if (!a) return set_error(MZS_E_ARG, "null arguments");
     if (a->dtype < MZS_DTYPE_FLOAT || a->dtype > MZS_DTYPE_HALF) return set_error(MZS_E_ARG, "logits: fp32, bf16 or fp16");
-    if (a->rows < 0 || a->n_actions < 1 || a->n_actions > 0x7fffffff) return set_error(MZS_E_ARG, "rows >= 0 and 1 <= n_actions < 2^31");
+    if (a->rows < 0 || a->n_actions < 1 || a->n_actions > (1 << 28)) return set_error(MZS_E_ARG, "rows >= 0 and 1 <= n_actions <= 2^28");
     if (a->top < 0 || a->top > MZS_POLICY_MAX_TOP) return set_error(MZS_E_ARG, "top: 0 .. MZS_POLICY_MAX_TOP");
     if (!(a->inverse_temperature > 0.0f) || a->inverse_temperature > 1e30f) return set_error(MZS_E_ARG, "inverse_temperature must be positive and finite");
     if (a->logits_stride < 0 || a->mask_stride < 0) return set_error(MZS_E_ARG, "negative row stride");
@@ -231,34 +762,131 @@ Row pack(const mzs_policy_args& a) {
     return p;
 }
 
-unsigned row_grid(int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
+constexpr int64_t kLanesMost = 2048; /* widest row of k_policy_lanes */
+
+/* how a wide row is cut: `chunks` blocks a row, each thread `vecs` vectors */
+struct Cut {
+    int chunks, vecs;
+};
+Cut cut_row(int64_t rows, int64_t n, int per, bool join) {
+    const int64_t all = (n + (int64_t)kBlock * per - 1) / ((int64_t)kBlock * per); /* vectors a thread would have of a whole row */
+    int64_t chunks = 1;
+    if (!join) chunks = (all + kAhead - 1) / kAhead;                                /* independent: four vectors a thread each */
+    else if (rows < 2048) chunks = (8192 + rows - 1) / rows;
+    if (join && chunks > kBlock) chunks = kBlock;
+    if (chunks > all) chunks = all;
+    Cut c;
+    c.vecs = (int)((all + chunks - 1) / chunks);
+    c.chunks = (int)((all + c.vecs - 1) / c.vecs);
+    return c;
+}
+
+template <typename T, bool kForward, bool kGrad>
+void launch_lanes(const Row& p, hipStream_t st) {
+    const auto go = [&](auto kernel, int per_block) {
+        const int64_t blocks = (p.rows + per_block - 1) / per_block;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(kBlock), 0, st, p);
+    };
+    if (p.n <= 4) go(k_policy_lanes<T, 1, 4, kForward, kGrad>, 256);
+    else if (p.n <= 16) go(k_policy_lanes<T, 4, 4, kForward, kGrad>, 64);
+    else if (p.n <= 64) go(k_policy_lanes<T, 16, 4, kForward, kGrad>, 16);
+    else if (p.n <= 256) go(k_policy_lanes<T, 16, 16, kForward, kGrad>, 16);
+    else if (p.n <= 1024) go(k_policy_lanes<T, 64, 16, kForward, kGrad>, 4);
+    else go(k_policy_lanes<T, 64, 32, kForward, kGrad>, 4);
+}
 
 template <typename T>
-void launch_rows(const Row& p, hipStream_t st) {
-    hipLaunchKernelGGL(k_policy_rows<T>, dim3(row_grid(p.rows)), dim3(kBlock), 0, st, p);
+void launch_forward(const Row& p, const mzs_policy_args& a, hipStream_t st) {
+    const Cut c = cut_row(p.rows, p.n, Kind<T>::kPer, true);
+    if (c.chunks == 1) {
+        hipLaunchKernelGGL((k_policy_chunk<T, false>), dim3((unsigned)p.rows), dim3(kBlock), 0, st, p, 1, c.vecs, nullptr, nullptr);
+        return;
+    }
+    float* parts = static_cast<float*>(a.workspace);
+    float* strips = parts + 3 * p.rows * c.chunks;
+    hipLaunchKernelGGL((k_policy_chunk<T, true>), dim3((unsigned)(p.rows * c.chunks)), dim3(kBlock), 0, st, p, c.chunks, c.vecs, parts, strips);
+    hipLaunchKernelGGL(k_policy_join<T>, dim3((unsigned)p.rows), dim3(kBlock), 0, st, p, c.chunks, c.vecs, (const float*)parts,
+                       (const float*)strips);
 }
 template <typename T>
-void launch_grad(const Row& p, hipStream_t st) {
-    hipLaunchKernelGGL(k_policy_grad<T>, dim3(row_grid(p.rows)), dim3(kBlock), 0, st, p);
+void launch_slope(const Row& p, hipStream_t st) {
+    const Cut c = cut_row(p.rows, p.n, Kind<T>::kPer, false);
+    hipLaunchKernelGGL(k_policy_slope<T>, dim3((unsigned)(p.rows * c.chunks)), dim3(kBlock), 0, st, p, c.chunks, c.vecs);
+}
+
+constexpr int kTrainThreads = 512, kTrainVecs = 24;
+template <typename T>
+bool fits_train(int64_t n) { return n <= (int64_t)kTrainThreads * kTrainVecs * Kind<T>::kPer; }
+template <typename T>
+void launch_train(const Row& p, hipStream_t st) {
+    const int64_t all = (p.n + (int64_t)kTrainThreads * Kind<T>::kPer - 1) / ((int64_t)kTrainThreads * Kind<T>::kPer);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.rows), dim3(kTrainThreads), 0, st, p); };
+    if (all <= 1) go(k_policy_train<T, kTrainThreads, 1>);
+    else if (all <= 2) go(k_policy_train<T, kTrainThreads, 2>);
+    else if (all <= 4) go(k_policy_train<T, kTrainThreads, 4>);
+    else if (all <= 8) go(k_policy_train<T, kTrainThreads, 8>);
+    else if (all <= 12) go(k_policy_train<T, kTrainThreads, 12>);
+    else if (all <= 16) go(k_policy_train<T, kTrainThreads, 16>);
+    else if (all <= 20) go(k_policy_train<T, kTrainThreads, 20>);
+    else go(k_policy_train<T, kTrainThreads, kTrainVecs>);
+}
+
+constexpr int64_t kSlab = 1 << 20; /* rows of a launch: blocks times threads stay below 2^32 */
+
+/* rows [r, r + rows) of a call */
+template <typename T>
+Row rows_from(Row p, int64_t r, int64_t rows) {
+    const auto on = [r](auto* q, int64_t each) { return q ? q + r * each : q; };
+    p.logits = on(static_cast<const T*>(p.logits), p.logits_stride);
+    p.mask = on(p.mask, p.mask_stride);
+    p.action = on(static_cast<const uint8_t*>(p.action), p.action_bytes);
+    p.log_prob = on(p.log_prob, 1), p.entropy = on(p.entropy, 1), p.log_z = on(p.log_z, 1), p.row_stats = on(p.row_stats, 2);
+    p.top_log_prob = on(p.top_log_prob, p.top), p.top_action = on(p.top_action, p.top);
+    p.grad_log_prob = on(p.grad_log_prob, 1), p.grad_entropy = on(p.grad_entropy, 1), p.grad_log_z = on(p.grad_log_z, 1);
+    p.grad_logits = on(static_cast<T*>(p.grad_logits), p.grad_stride);
+    p.rows = rows;
+    return p;
+}
+template <typename T>
+void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool forward, bool grad) {
+    if (all.n <= kLanesMost) {
+        if (forward && grad) launch_lanes<T, true, true>(all, st);
+        else if (forward) launch_lanes<T, true, false>(all, st);
+        else launch_lanes<T, false, true>(all, st);
+        return;
+    }
+    for (int64_t r = 0; r < all.rows; r += kSlab) {
+        const Row p = rows_from<T>(all, r, all.rows - r < kSlab ? all.rows - r : kSlab);
+        if (forward && grad && fits_train<T>(p.n)) {
+            launch_train<T>(p, st);
+            continue;
+        }
+        if (forward) launch_forward<T>(p, a, st);
+        if (grad) launch_slope<T>(p, st);
+    }
+}
+
+size_t workspace_bytes(const mzs_policy_args& a, int per) {
+    if (a.rows == 0 || a.n_actions <= kLanesMost) return 0;
+    const Cut c = cut_row(a.rows, a.n_actions, per, true);
+    if (c.chunks == 1) return 0;
+    return sizeof(float) * (size_t)a.rows * c.chunks * (3 + (a.top > 0 ? kBlock : 0));
 }
 
 int run(const mzs_policy_args* a, void* stream, bool forward, bool grad) {
     const int rc = check(a, forward, grad);
     if (rc || a->rows == 0) return rc;
+    if (forward) {
+        const size_t need = workspace_bytes(*a, a->dtype == MZS_DTYPE_FLOAT ? 4 : 8);
+        if (need && (!a->workspace || a->workspace_bytes < need)) return set_error(MZS_E_ARG, "workspace too small (mzs_policy_workspace)");
+    }
     DeviceScope scope(a->device);
     if (scope.status != hipSuccess) return hip_error("mzs_policy: device", scope.status);
     const Row p = pack(*a);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (forward) {
-        if (a->dtype == MZS_DTYPE_FLOAT) launch_rows<float>(p, st);
-        else if (a->dtype == MZS_DTYPE_BFLOAT) launch_rows<bf16>(p, st);
-        else launch_rows<_Float16>(p, st);
-    }
-    if (grad) {
-        if (a->dtype == MZS_DTYPE_FLOAT) launch_grad<float>(p, st);
-        else if (a->dtype == MZS_DTYPE_BFLOAT) launch_grad<bf16>(p, st);
-        else launch_grad<_Float16>(p, st);
-    }
+    if (a->dtype == MZS_DTYPE_FLOAT) run_kind<float>(p, *a, st, forward, grad);
+    else if (a->dtype == MZS_DTYPE_BFLOAT) run_kind<__bf16>(p, *a, st, forward, grad);
+    else run_kind<_Float16>(p, *a, st, forward, grad);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? MZS_OK : hip_error("mzs_policy: launch", e);
 }
@@ -270,7 +898,9 @@ extern "C" {
 
 int mzs_policy_workspace(const mzs_policy_args* args, size_t* bytes_out) {
     if (!args || !bytes_out) return mzs::set_error(MZS_E_ARG, "null argument");
-    *bytes_out = 0;
+    if (args->dtype < MZS_DTYPE_FLOAT || args->dtype > MZS_DTYPE_HALF || args->rows < 0 || args->n_actions < 1 || args->n_actions > (1 << 28))
+        return mzs::set_error(MZS_E_ARG, "fp32, bf16 or fp16; rows >= 0 and 1 <= n_actions <= 2^28");
+    *bytes_out = mzs::workspace_bytes(*args, args->dtype == MZS_DTYPE_FLOAT ? 4 : 8);
     return MZS_OK;
 }
 int mzs_policy_log_probs(const mzs_policy_args* args, void* stream) { return mzs::run(args, stream, true, false); }

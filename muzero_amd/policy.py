@@ -35,8 +35,8 @@ def _check(logits, actions, mask, temperature, top):
     if logits.dtype not in _DTYPES:
         raise ValueError(f"logits are {logits.dtype}: float32, bfloat16 or float16")
     n = logits.shape[-1]
-    if not 1 <= n < 2 ** 31:
-        raise ValueError(f"{n} actions: 1 .. 2^31 - 1")
+    if not 1 <= n <= 2 ** 28:
+        raise ValueError(f"{n} actions: 1 .. 2^28")
     if not 1e-30 <= temperature < float("inf"):
         raise ValueError(f"temperature={temperature!r}: positive and finite (at least 1e-30)")
     if not 0 <= top <= _lib.POLICY_MAX_TOP:
