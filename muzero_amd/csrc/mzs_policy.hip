@@ -265,7 +265,7 @@ __device__ __forceinline__ float slope_at(const Row& p, const Slope& q, float x)
 /* ------------------------------------------------------------------ narrow rows
  * G lanes hold a row of up to G * E logits in registers, 64 / G rows to a wave: one read, one write, no shared memory.  The choice of
  * G and E by n is in launch_lanes. */
-template <typename T, int G, int E, bool kForward, bool kGrad>
+template <typename T, int G, int E, bool kForward, bool kGrad, bool kTop>
 __global__ void __launch_bounds__(kBlock) k_policy_lanes(const Row p) {
     constexpr int kRows = kBlock / G;
     const int g = threadIdx.x % G;
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kBlock) k_policy_lanes(const Row p) {
         if (v.big == kInf) v.s = __builtin_nanf("");
         const Values o = row_values(p, v);
         if (kForward && live && g == 0) write_row(p, r, v, o, la, a);
-        if (kForward && p.top > 0) {
+        if (kTop) {
             uint32_t key[E];
             _Pragma("unroll") for (int j = 0; j < E; ++j)
                 key[j] = x[j] == -kInf ? 0u : (uint32_t)(rank_key(x[j], 0) >> 32);
@@ -342,52 +342,66 @@ __global__ void __launch_bounds__(kBlock) k_policy_lanes(const Row p) {
 /* ------------------------------------------------------------------ wide rows
  * A block walks a chunk of a row: thread t takes the 16-byte vectors t, t + kBlock, ... of it. */
 
-/* merges every thread's part; all threads return the whole.  lds: 3 floats a wave */
+/* largest value over the block, in every thread.  lds: a float a wave */
 template <int kThreads>
-__device__ __forceinline__ Sum block_merge(const Row& p, Sum v, float* lds) {
+__device__ __forceinline__ float block_max(float v, float* lds) {
+    v = lanes_max<64>(v);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    _Pragma("unroll") for (int w = 0; w < kThreads / 64; ++w) v = fmaxf(v, lds[w]);
+    return v;
+}
+/* s and t, relative to the block's maximum, summed over the block, in every thread.  lds: two floats a wave, others than block_max's */
+template <int kThreads>
+__device__ __forceinline__ Sum block_sum(float big, float s, float t, float* lds) {
     constexpr int kWaves = kThreads / 64;
-    const int wave = threadIdx.x >> 6;
-    float big = lanes_max<64>(v.big);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[wave] = big;
-    __syncthreads();
-    _Pragma("unroll") for (int w = 0; w < kWaves; ++w) big = fmaxf(big, lds[w]);
-    const float d = v.big == big ? 0.0f : fmaxf(p.c * (v.big - big), kLow), f = __builtin_amdgcn_exp2f(d);
-    const float s = lanes_sum<64>(f * v.s), t = lanes_sum<64>(f * (v.t + d * v.s));
-    if ((threadIdx.x & 63) == 0) lds[kWaves + wave] = s, lds[2 * kWaves + wave] = t;
+    s = lanes_sum<64>(s), t = lanes_sum<64>(t);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s, lds[kWaves + (threadIdx.x >> 6)] = t;
     __syncthreads();
     Sum o{big, 0.0f, 0.0f};
-    _Pragma("unroll") for (int w = 0; w < kWaves; ++w) o.s += lds[kWaves + w], o.t += lds[2 * kWaves + w];
+    _Pragma("unroll") for (int w = 0; w < kWaves; ++w) o.s += lds[w], o.t += lds[kWaves + w];
     if (big == kInf) o.s = __builtin_nanf("");
     return o;
+}
+/* merges every thread's part; all threads return the whole.  lds: three floats a wave */
+template <int kThreads>
+__device__ __forceinline__ Sum block_merge(const Row& p, Sum v, float* lds) {
+    const float big = block_max<kThreads>(v.big, lds);
+    const float d = v.big == big ? 0.0f : fmaxf(p.c * (v.big - big), kLow), f = __builtin_amdgcn_exp2f(d);
+    return block_sum<kThreads>(big, f * v.s, f * (v.t + d * v.s), lds + kThreads / 64);
 }
 
 constexpr int kAhead = 4; /* vectors a thread has in flight */
 
-/* The compiler may not look behind this: a row held packed is unpacked anew in each pass over it, a vector at a time, where it would
- * otherwise keep every unpacked value (twice the registers, which spill). */
+/* The compiler may not look behind this: a row held packed is unpacked anew in each pass over it, where it would otherwise keep every
+ * unpacked value (twice the registers, which spill). */
 __device__ __forceinline__ void unpack_here(w4& v) { asm volatile("" : "+v"(v)); }
 
-/* takes kPer * N logits into a thread's running sum: their maximum first, one rescaling, then the exponentials */
 template <typename T, int N>
-__device__ __forceinline__ void sum_vecs(const Row& p, w4* v, Sum& sum) {
-    constexpr int kPer = Kind<T>::kPer;
-    float big = sum.big;
-    _Pragma("unroll") for (int u = 0; u < N; ++u) {
-        if (N > kAhead) unpack_here(v[u]);
-        _Pragma("unroll") for (int j = 0; j < kPer; ++j) big = fmaxf(big, Kind<T>::get(v[u], j));
-    }
+__device__ __forceinline__ float max_vecs(const w4* v, float big) {
+    _Pragma("unroll") for (int u = 0; u < N; ++u)
+        _Pragma("unroll") for (int j = 0; j < Kind<T>::kPer; ++j) big = fmaxf(big, Kind<T>::get(v[u], j));
+    return big;
+}
+/* adds the exponentials relative to `ref`, a finite number (or one whose row is NaN anyway) that no logit exceeds */
+template <typename T, int N>
+__device__ __forceinline__ void sum_vecs(const Row& p, const w4* v, float ref, float& s, float& t) {
+    _Pragma("unroll") for (int u = 0; u < N; ++u)
+        _Pragma("unroll") for (int j = 0; j < Kind<T>::kPer; ++j) {
+            const float d = p.c * (Kind<T>::get(v[u], j) - ref), e = __builtin_amdgcn_exp2f(d);
+            s += e, t = fmaf(e, fmaxf(d, kLow), t);
+        }
+}
+/* nothing allowed: relative to 0 every exponential is 0 (or NaN) */
+__device__ __forceinline__ float reference(float big) { return big == -kInf ? 0.0f : big; }
+
+/* takes N vectors into a thread's running sum: their maximum first, one rescaling, then the exponentials */
+template <typename T, int N>
+__device__ __forceinline__ void take_vecs(const Row& p, const w4* v, Sum& sum) {
+    const float big = max_vecs<T, N>(v, sum.big);
     const float shift = sum.big == big ? 0.0f : fmaxf(p.c * (sum.big - big), kLow), f = __builtin_amdgcn_exp2f(shift);
     float s = f * sum.s, t = f * (sum.t + shift * sum.s);
-    const float ref = big == -kInf ? 0.0f : big; /* nothing allowed so far: every exponential is 0 (or NaN) */
-    _Pragma("unroll") for (int u = 0; u < N; ++u) {
-        if (N > kAhead) unpack_here(v[u]);
-        _Pragma("unroll") for (int j = 0; j < kPer; ++j) {
-            const float x = Kind<T>::get(v[u], j);
-            const float d0 = p.c * (x - ref), e = __builtin_amdgcn_exp2f(d0);
-            s += e, t = fmaf(e, fmaxf(d0, kLow), t);
-        }
-    }
+    sum_vecs<T, N>(p, v, reference(big), s, t);
     sum = Sum{big, s, t};
 }
 
@@ -581,11 +595,11 @@ __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks
     for (; j + kAhead <= chunk_vecs; j += kAhead) {
         w4 x[kAhead];
         load_vecs<T, kAhead>(l, mask, from + (uint32_t)j * kBlock * kPer, kBlock * kPer, n, x);
-        sum_vecs<T, kAhead>(p, x, v);
+        take_vecs<T, kAhead>(p, x, v);
     }
     for (; j < chunk_vecs; ++j) {
         w4 x = load_vec<T>(l, mask, from + (uint32_t)j * kBlock * kPer, n);
-        sum_vecs<T, 1>(p, &x, v);
+        take_vecs<T, 1>(p, &x, v);
     }
     const float mine = v.big;
     v = block_merge<kBlock>(p, v, lds);
@@ -686,42 +700,40 @@ __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks
     }
 }
 
-/* Forward and gradient of a row that a block holds in registers (V 16-byte vectors a thread): one read and one write of memory. */
+/* Forward and gradient of a row that a block holds in registers (V 16-byte vectors a thread): one read and one write of memory.  Without
+ * alternatives: their search would hold its registers on top of the row's. */
 template <typename T, int kThreads, int V>
-__global__ void __launch_bounds__(kThreads) k_policy_train(const Row p) {
+__global__ void __launch_bounds__(kThreads, 4) k_policy_train(const Row p) {
     constexpr int kPer = Kind<T>::kPer;
     __shared__ float lds[3 * (kThreads / 64)];
-    __shared__ float maxima[kThreads];
-    __shared__ TopScratch top;
     const int64_t r = blockIdx.x;
     const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
     const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
-    const uint32_t n = (uint32_t)p.n, from = threadIdx.x * kPer;
+    const uint32_t n = (uint32_t)p.n;
+    uint32_t from = threadIdx.x * kPer;
     w4 x[V];
-    constexpr int kGroup = V < kAhead ? V : kAhead;
-    static_assert(V % kGroup == 0, "whole groups");
-    _Pragma("unroll") for (int j = 0; j < V; j += kGroup)
-        load_vecs<T, kGroup>(l, mask, from + j * kThreads * kPer, kThreads * kPer, n, x + j);
+    constexpr int kGroups = V / kAhead;
+    _Pragma("unroll") for (int j = 0; j < kGroups; ++j)
+        load_vecs<T, kAhead>(l, mask, from + j * kAhead * kThreads * kPer, kThreads * kPer, n, x + j * kAhead);
+    if constexpr (V % kAhead != 0)
+        load_vecs<T, V % kAhead>(l, mask, from + kGroups * kAhead * kThreads * kPer, kThreads * kPer, n, x + kGroups * kAhead);
     const int64_t a = row_action(p, r);
     const float la = action_logit<T>(p, l, mask, a); /* before the gradient may overwrite it */
-    Sum v{-kInf, 0.0f, 0.0f};
-    sum_vecs<T, V>(p, x, v);
-    const float mine = v.big;
-    v = block_merge<kThreads>(p, v, lds);
+    _Pragma("unroll") for (int j = 0; j < V; ++j) unpack_here(x[j]);
+    const float big = block_max<kThreads>(max_vecs<T, V>(x, -kInf), lds);
+    _Pragma("unroll") for (int j = 0; j < V; ++j) unpack_here(x[j]);
+    float s = 0.0f, t = 0.0f;
+    sum_vecs<T, V>(p, x, reference(big), s, t);
+    const Sum v = block_sum<kThreads>(big, s, t, lds + kThreads / 64);
     const Values o = row_values(p, v);
     if (threadIdx.x == 0) write_row(p, r, v, o, la, a);
-    if (p.top > 0) {
-        maxima[threadIdx.x] = mine;
-        __syncthreads();
-        select_top<T, kThreads>(p, r, l, mask, v, o, [&](int i) { return maxima[i]; }, kThreads, V, (uint32_t)V * kThreads * kPer, top);
-        __syncthreads();
-    }
     const Slope q = row_slope(p, r, a, v, o.entropy, o.log2_s);
     T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
     const uint32_t action = a >= 0 && a < p.n ? (uint32_t)a : ~0u;
+    asm volatile("" : "+v"(from)); /* the places are worked out anew, not kept since the loads */
     _Pragma("unroll") for (int j = 0; j < V; ++j) {
         const uint32_t i = from + j * kThreads * kPer;
-        if (V > kAhead) unpack_here(x[j]);
+        unpack_here(x[j]);
         store_vec<T>(out, i, n, q.empty ? w4{0, 0, 0, 0} : slope_vec<T>(p, q, x[j], i, action));
     }
 }
@@ -762,7 +774,7 @@ Row pack(const mzs_policy_args& a) {
     return p;
 }
 
-constexpr int64_t kLanesMost = 2048; /* widest row of k_policy_lanes */
+constexpr int64_t kLanesMost = 1024; /* widest row of k_policy_lanes */
 
 /* how a wide row is cut: `chunks` blocks a row, each thread `vecs` vectors */
 struct Cut {
@@ -781,18 +793,17 @@ Cut cut_row(int64_t rows, int64_t n, int per, bool join) {
     return c;
 }
 
-template <typename T, bool kForward, bool kGrad>
+template <typename T, bool kForward, bool kGrad, bool kTop>
 void launch_lanes(const Row& p, hipStream_t st) {
     const auto go = [&](auto kernel, int per_block) {
         const int64_t blocks = (p.rows + per_block - 1) / per_block;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(kBlock), 0, st, p);
     };
-    if (p.n <= 4) go(k_policy_lanes<T, 1, 4, kForward, kGrad>, 256);
-    else if (p.n <= 16) go(k_policy_lanes<T, 4, 4, kForward, kGrad>, 64);
-    else if (p.n <= 64) go(k_policy_lanes<T, 16, 4, kForward, kGrad>, 16);
-    else if (p.n <= 256) go(k_policy_lanes<T, 16, 16, kForward, kGrad>, 16);
-    else if (p.n <= 1024) go(k_policy_lanes<T, 64, 16, kForward, kGrad>, 4);
-    else go(k_policy_lanes<T, 64, 32, kForward, kGrad>, 4);
+    if (p.n <= 4) go(k_policy_lanes<T, 1, 4, kForward, kGrad, kTop>, 256);
+    else if (p.n <= 16) go(k_policy_lanes<T, 4, 4, kForward, kGrad, kTop>, 64);
+    else if (p.n <= 64) go(k_policy_lanes<T, 16, 4, kForward, kGrad, kTop>, 16);
+    else if (p.n <= 256) go(k_policy_lanes<T, 16, 16, kForward, kGrad, kTop>, 16);
+    else go(k_policy_lanes<T, 64, 16, kForward, kGrad, kTop>, 4);
 }
 
 template <typename T>
@@ -828,6 +839,7 @@ void launch_train(const Row& p, hipStream_t st) {
     else if (all <= 12) go(k_policy_train<T, kTrainThreads, 12>);
     else if (all <= 16) go(k_policy_train<T, kTrainThreads, 16>);
     else if (all <= 20) go(k_policy_train<T, kTrainThreads, 20>);
+    else if (all <= 21) go(k_policy_train<T, kTrainThreads, 21>);
     else go(k_policy_train<T, kTrainThreads, kTrainVecs>);
 }
 
@@ -850,14 +862,15 @@ Row rows_from(Row p, int64_t r, int64_t rows) {
 template <typename T>
 void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool forward, bool grad) {
     if (all.n <= kLanesMost) {
-        if (forward && grad) launch_lanes<T, true, true>(all, st);
-        else if (forward) launch_lanes<T, true, false>(all, st);
-        else launch_lanes<T, false, true>(all, st);
+        if (forward && all.top > 0) launch_lanes<T, true, false, true>(all, st);
+        else if (forward && !grad) launch_lanes<T, true, false, false>(all, st);
+        else if (forward) launch_lanes<T, true, true, false>(all, st);
+        if (grad && (!forward || all.top > 0)) launch_lanes<T, false, true, false>(all, st);
         return;
     }
     for (int64_t r = 0; r < all.rows; r += kSlab) {
         const Row p = rows_from<T>(all, r, all.rows - r < kSlab ? all.rows - r : kSlab);
-        if (forward && grad && fits_train<T>(p.n)) {
+        if (forward && grad && p.top == 0 && fits_train<T>(p.n)) {
             launch_train<T>(p, st);
             continue;
         }

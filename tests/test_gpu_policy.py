@@ -115,6 +115,9 @@ def check(logits, actions=None, mask=None, temperature=1.0, top=0, seed=0):
     auto, = torch.autograd.grad([o for o, _ in roots], leaf, [u for _, u in roots])
     both, joined = policy_log_probs_grad(logits, actions, *up, mask=mask, temperature=temperature, top=top)
     plain = policy_log_probs(logits.detach(), actions, mask=mask, temperature=temperature, top=top)
+    if top:         # with and without alternatives are two ways
+        _, alone = policy_log_probs_grad(logits, actions, *up, mask=mask, temperature=temperature)
+        close(alone, *exact_grad(e, actions, *up, temperature, logits.dtype), "gradient without alternatives")
     want, tol = exact_grad(e, actions, *up, temperature, logits.dtype)
     for name, o in (("forward", out), ("joined", both), ("no grad", plain)):
         close(o.log_z, e["log_z"], e["tol_z"], name + " log_z")
