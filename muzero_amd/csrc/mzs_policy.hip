@@ -405,98 +405,84 @@ __device__ __forceinline__ void take_vecs(const Row& p, const w4* v, Sum& sum) {
     sum = Sum{big, s, t};
 }
 
-constexpr int kHistogram = 256;
-constexpr int kStrips = 512;  /* strips that can hold alternatives              */
-constexpr int kKeys = 1024;   /* logits that can be alternatives                */
+constexpr int kStrips = 512; /* strips that can hold alternatives              */
+constexpr int kKeys = 1024;  /* logits that can be alternatives                */
+constexpr int kGroups = kBlock / 4; /* four threads' strips: enough groups for MZS_POLICY_MAX_TOP of them */
+static_assert(kBlock / 64 <= kGroups && MZS_POLICY_MAX_TOP <= kGroups, "tau is one of the groups' maxima");
 struct TopScratch {
-    uint32_t histogram[kHistogram];
-    uint32_t strips[kStrips];
     uint64_t keys[kKeys];
-    uint32_t n_strips, n_keys, bin, rest;
-    uint64_t best[kBlock / 64 * 4];
+    uint32_t strips[kStrips];
+    alignas(16) uint32_t groups[kGroups];
+    uint32_t n_strips, n_keys, tau;
+    uint64_t best[kBlock / 64];
 };
 
+/* order of logits as unsigned numbers, 0 for what is not allowed */
 __device__ __forceinline__ uint32_t rank_value(float x) { return x == -kInf ? 0u : (uint32_t)(rank_key(x, 0) >> 32); }
 
-/* A strip: the vectors that one thread took of one chunk, with the largest of their logits.  The `top` largest logits of a row lie at or
- * above the top-th largest strip maximum tau (that many strips have one there), so:
- *   1. tau from a radix selection over the strips' maxima, 8 bits of the ordered value a pass;
- *   2. strips whose maximum reaches tau are read again, logits that reach it are collected;
- *   3. a collected logit's rank is the number of collected ones before it.
- * After two passes tau is known to 16 bits, which collects little more than it has to — unless many logits are alike.  Then the selection
- * goes on to all 32 bits, logits above tau are collected (there are fewer than `top` strips of them), and the ones equal
- * to tau are taken from the row's start on.  A row where even that is too much (or with NaN) is searched `top` times. */
-template <typename T, int kThreads, typename Maximum>
-__device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* mask, const Sum& v, const Values& o, Maximum maximum,
+constexpr int kStripLanes = 4;                     /* neighbouring threads whose vectors make a strip */
+constexpr int kStripsPerBlock = kBlock / kStripLanes;
+static_assert(kStripsPerBlock == kBlock / 4 && kStripLanes == 4, "held_strip gives a lone chunk its own threads");
+constexpr int kHold = 16; /* strips of a row that a thread holds in registers */
+/* strip in held[h] of this thread; >= n_strips: none.  Few strips are spread over the block, so that every group has one. */
+__device__ __forceinline__ int held_strip(int h, int n_strips) {
+    const int spread = n_strips <= kBlock / 4 ? 4 : n_strips <= kBlock / 2 ? 2 : 1;
+    const int at = threadIdx.x + h * kBlock;
+    return at % spread ? n_strips : at / spread;
+}
+
+/* Alternatives from strips.  A strip is the vectors that kStripLanes threads took of one chunk; its largest logit is known.  Each four of
+ * the block's threads take the largest over their share of the strips; tau, the top-th largest of those 64, is reached by at least `top`
+ * logits, so
+ *   1. strips whose maximum reaches tau are read again and their logits that reach it collected — hardly more than `top` of them, as
+ *      the best ones seldom share a group (top 20: 24 on the average, top 32: 44);
+ *   2. a collected logit's rank is the number of collected ones before it.
+ * Both need little more than the strips' maxima (1 / 64 of the row or less), whatever the logits — unless many are alike: where they do not
+ * fit the lists, only those above tau are collected, and the ones equal to tau are taken from the row's start on.  A row where
+ * even that is too much (or with NaN) is searched `top` times.  Every choice is by value and index: the lists' order does not matter. */
+template <typename T, typename Maximum>
+__device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* mask, const Sum& v, const Values& o, const float* held, Maximum maximum,
                            int n_strips, int chunk_vecs, uint32_t chunk_len, TopScratch& sh) {
     constexpr int kPer = Kind<T>::kPer;
     const int tid = threadIdx.x;
-    const uint32_t want = (uint32_t)p.top;
-    const uint32_t n = (uint32_t)p.n;
-    uint32_t tau = 0, fixed = 0; /* the bits of tau known so far, and which */
-    bool done = false;
+    const uint32_t want = (uint32_t)p.top, n = (uint32_t)p.n;
     const bool plain = v.s == v.s;
+    uint32_t mine = 0;
+    _Pragma("unroll") for (int h = 0; h < kHold; ++h) mine = max(mine, rank_value(held[h]));
+    for (int i = tid + kHold * kBlock; i < n_strips; i += kBlock) mine = max(mine, rank_value(maximum(i)));
+    uint32_t group = max(mine, (uint32_t)__builtin_amdgcn_mov_dpp((int)mine, 0xB1, 0xf, 0xf, true));
+    group = max(group, (uint32_t)__builtin_amdgcn_mov_dpp((int)group, 0x4E, 0xf, 0xf, true));
+    if (tid % 4 == 0) sh.groups[tid / 4] = group;
+    if (tid == 0) sh.tau = 0xffffffffu;
+    __syncthreads();
+    uint32_t ahead = 0; /* groups with a larger one */
+    _Pragma("unroll") for (int i = 0; i < kGroups / 4; ++i) {
+        const w4 g = *reinterpret_cast<const w4*>(sh.groups + 4 * i);
+        _Pragma("unroll") for (int j = 0; j < 4; ++j) ahead += g[j] > group;
+    }
+    if (ahead < want) atomicMin(&sh.tau, group); /* the smallest of those that fewer than `top` are ahead of */
+    bool done = false;
     for (int stage = 0; stage < 2 && plain && !done; ++stage) {
-        uint32_t left = want;
-        if (stage) { /* go on from the 16 bits: how many strips are above them */
-            if (tid == 0) sh.rest = 0;
-            __syncthreads();
-            uint32_t above = 0;
-            for (int i = tid; i < n_strips; i += kThreads) above += (rank_value(maximum(i)) & fixed) > tau;
-            if (above) atomicAdd(&sh.rest, above);
-            __syncthreads();
-            left = want > sh.rest ? want - sh.rest : 1u;
-            __syncthreads();
-        }
-        for (int pass = 2 * stage; pass < 2 * stage + 2; ++pass) {
-            const int shift = 24 - 8 * pass;
-            for (int i = tid; i < kHistogram; i += kThreads) sh.histogram[i] = 0;
-            __syncthreads();
-            for (int i = tid; i < n_strips; i += kThreads) {
-                const uint32_t k = rank_value(maximum(i));
-                if (k && (k & fixed) == tau) atomicAdd(&sh.histogram[(k >> shift) & 255u], 1u);
-            }
-            __syncthreads();
-            if (tid < 64) { /* lane i: bins 4 i .. 4 i + 3; counts from the top */
-                uint32_t c[4], mine = 0;
-                for (int j = 0; j < 4; ++j) mine += c[j] = sh.histogram[4 * tid + j];
-                uint32_t above = mine;
-                for (int off = 1; off < 64; off <<= 1) {
-                    const uint32_t other = __shfl_down(above, off, 64);
-                    if (tid + off < 64) above += other;
-                }
-                above -= mine; /* strips in the bins of higher lanes */
-                if (tid == 0) sh.bin = 0, sh.rest = left;
-                __builtin_amdgcn_wave_barrier();
-                if (above < left && above + mine >= left) {
-                    uint32_t higher = above;
-                    for (int j = 3; j >= 0; --j) {
-                        if (higher < left && higher + c[j] >= left) sh.bin = 4 * tid + j, sh.rest = left - higher;
-                        higher += c[j];
-                    }
-                }
-            }
-            __syncthreads();
-            tau |= sh.bin << shift, fixed |= 255u << shift;
-            left = sh.rest;
-            __syncthreads();
-        }
-        /* strips and logits at or above tau (second stage: above) */
+        __syncthreads();
+        const uint32_t tau = sh.tau, least = stage ? tau + 1u : max(tau, 1u);
         if (tid == 0) sh.n_strips = 0, sh.n_keys = 0;
         __syncthreads();
-        const uint32_t least = stage ? tau + 1u : tau > 0u ? tau : 1u;
-        for (int i = tid; i < n_strips; i += kThreads)
-            if (rank_value(maximum(i)) >= least) {
+        const auto look = [&](float largest, int i) {
+            if (rank_value(largest) >= least) {
                 const uint32_t at = atomicAdd(&sh.n_strips, 1u);
                 if (at < kStrips) sh.strips[at] = i;
             }
+        };
+        if (mine >= least) {
+            _Pragma("unroll") for (int h = 0; h < kHold; ++h) look(held[h], held_strip(h, n_strips));
+            for (int i = tid + kHold * kBlock; i < n_strips; i += kBlock) look(maximum(i), i);
+        }
         __syncthreads();
-        const uint32_t found = sh.n_strips;
+        const uint32_t found = sh.n_strips, each = (uint32_t)chunk_vecs * kStripLanes;
         if (found <= kStrips) {
-            for (uint32_t w = tid; w < found * chunk_vecs; w += kThreads) {
-                const uint32_t strip = sh.strips[w / chunk_vecs], j = w % chunk_vecs;
-                const uint32_t chunk = strip / kThreads, t = strip % kThreads;
-                const uint32_t i = chunk * chunk_len + (j * kThreads + t) * kPer; /* below n rounded up to a chunk's vectors: 32 bits */
+            for (uint32_t w = tid; w < found * each; w += kBlock) {
+                const uint32_t strip = sh.strips[w / each], lane = w % kStripLanes, j = w % each / kStripLanes;
+                const uint32_t i = strip / kStripsPerBlock * chunk_len + (j * kBlock + strip % kStripsPerBlock * kStripLanes + lane) * kPer;
                 if (i >= n) continue;
                 const w4 x = load_vec<T>(l, mask, i, n);
                 _Pragma("unroll") for (int q = 0; q < kPer; ++q) {
@@ -512,56 +498,55 @@ __device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* m
         const uint32_t n_keys = sh.n_keys;
         done = found <= kStrips && n_keys <= kKeys;
         if (done) {
-            for (uint32_t i = tid; i < n_keys; i += kThreads) {
+            for (uint32_t i = tid; i < n_keys; i += kBlock) {
                 const uint64_t key = sh.keys[i];
                 uint32_t rank = 0;
                 for (uint32_t k = 0; k < n_keys; ++k) rank += sh.keys[k] > key;
                 if (rank < want) write_top(p, r, rank, key, v, o);
             }
-            uint32_t at = n_keys < want ? n_keys : want;
+            uint32_t at = min(n_keys, want);
             if (stage && tau) { /* equal ones in the row's order */
-                for (uint32_t i0 = 0; i0 < n && at < want; i0 += kThreads * kPer) {
+                for (uint32_t i0 = 0; i0 < n && at < want; i0 += kBlock * kPer) {
                     const uint32_t i = i0 + tid * kPer;
                     uint32_t hit = 0;
                     if (i < n) {
                         const w4 x = load_vec<T>(l, mask, i, n);
                         _Pragma("unroll") for (int q = 0; q < kPer; ++q) hit |= (uint32_t)(rank_value(Kind<T>::get(x, q)) == tau) << q;
                     }
-                    uint32_t before = __popc(hit);
-                    const uint32_t mine = before;
+                    const uint32_t count = __popc(hit);
+                    uint32_t up_to = count;
                     for (int off = 1; off < 64; off <<= 1) {
-                        const uint32_t other = __shfl_up(before, off, 64);
-                        if ((tid & 63) >= off) before += other;
+                        const uint32_t other = __shfl_up(up_to, off, 64);
+                        if ((tid & 63) >= off) up_to += other;
                     }
-                    if ((tid & 63) == 63) sh.histogram[tid >> 6] = before;
+                    if ((tid & 63) == 63) sh.groups[tid >> 6] = up_to;
                     __syncthreads();
-                    uint32_t slot = at + before - mine, all = 0;
-                    for (int w = 0; w < kThreads / 64; ++w) {
-                        if (w < (tid >> 6)) slot += sh.histogram[w];
-                        all += sh.histogram[w];
+                    uint32_t slot = at + up_to - count, all = 0;
+                    for (int w = 0; w < kBlock / 64; ++w) {
+                        if (w < (tid >> 6)) slot += sh.groups[w];
+                        all += sh.groups[w];
                     }
                     for (int q = 0; q < kPer; ++q)
                         if ((hit >> q) & 1u) {
-                            if (slot < want) write_top(p, r, slot, ((uint64_t)tau << 32) | (0xffffffffu - (uint32_t)(i + q)), v, o);
+                            if (slot < want) write_top(p, r, slot, ((uint64_t)tau << 32) | (0xffffffffu - (i + q)), v, o);
                             ++slot;
                         }
-                    at = at + all < want ? at + all : want;
+                    at = min(at + all, want);
                     __syncthreads();
                 }
             }
-            for (uint32_t k = at + tid; k < want; k += kThreads) write_top(p, r, k, 0, v, o);
+            for (uint32_t k = at + tid; k < want; k += kBlock) write_top(p, r, k, 0, v, o);
         }
-        __syncthreads();
     }
     if (done) return;
     uint64_t last = ~0ull;
     for (uint32_t k = 0; k < want; ++k) {
         uint64_t best = 0;
-        for (uint32_t i = tid * kPer; i < n; i += kThreads * kPer) {
+        for (uint32_t i = tid * kPer; i < n; i += kBlock * kPer) {
             const w4 x = load_vec<T>(l, mask, i, n);
             _Pragma("unroll") for (int q = 0; q < kPer; ++q) {
                 const uint32_t c = rank_value(Kind<T>::get(x, q));
-                const uint64_t key = c ? ((uint64_t)c << 32) | (0xffffffffu - (uint32_t)(i + q)) : 0;
+                const uint64_t key = c ? ((uint64_t)c << 32) | (0xffffffffu - (i + q)) : 0;
                 if (key < last && key > best) best = key;
             }
         }
@@ -569,12 +554,12 @@ __device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* m
             const uint64_t other = __shfl_xor((unsigned long long)best, off, 64);
             best = other > best ? other : best;
         }
+        __syncthreads();
         if ((tid & 63) == 0) sh.best[tid >> 6] = best;
         __syncthreads();
-        for (int w = 0; w < kThreads / 64; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+        for (int w = 0; w < kBlock / 64; ++w) best = max(best, sh.best[w]);
         last = best;
         if (tid == 0) write_top(p, r, k, last, v, o);
-        __syncthreads();
     }
 }
 
@@ -590,6 +575,8 @@ __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks
     const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
     const uint32_t n = (uint32_t)p.n;
     const uint32_t chunk_len = (uint32_t)chunk_vecs * kBlock * kPer, from = chunk * chunk_len + threadIdx.x * kPer;
+    const int64_t a = kSplit ? -1 : row_action(p, r); /* asked for early: nothing waits for it behind the sums */
+    const float la = kSplit ? 0.0f : action_logit<T>(p, l, mask, a);
     Sum v{-kInf, 0.0f, 0.0f};
     int j = 0;
     for (; j + kAhead <= chunk_vecs; j += kAhead) {
@@ -601,26 +588,24 @@ __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks
         w4 x = load_vec<T>(l, mask, from + (uint32_t)j * kBlock * kPer, n);
         take_vecs<T, 1>(p, &x, v);
     }
-    const float mine = v.big;
+    const float strip = lanes_max<kStripLanes>(v.big);
     v = block_merge<kBlock>(p, v, lds);
     if constexpr (kSplit) {
-        if (p.top > 0) strips[(int64_t)blockIdx.x * kBlock + threadIdx.x] = mine;
+        if (p.top > 0 && threadIdx.x % kStripLanes == 0)
+            strips[(int64_t)blockIdx.x * kStripsPerBlock + threadIdx.x / kStripLanes] = strip;
         if (threadIdx.x == 0) {
             float* q = parts + 3 * (int64_t)blockIdx.x;
             q[0] = v.big, q[1] = v.s, q[2] = v.t;
         }
     } else {
-        __shared__ float maxima[kBlock];
         __shared__ TopScratch top;
         const Values o = row_values(p, v);
-        if (threadIdx.x == 0) {
-            const int64_t a = row_action(p, r);
-            write_row(p, r, v, o, action_logit<T>(p, l, mask, a), a);
-        }
+        if (threadIdx.x == 0) write_row(p, r, v, o, la, a);
         if (p.top > 0) {
-            maxima[threadIdx.x] = mine;
-            __syncthreads();
-            select_top<T, kBlock>(p, r, l, mask, v, o, [&](int i) { return maxima[i]; }, kBlock, chunk_vecs, chunk_len, top);
+            float held[kHold];
+            _Pragma("unroll") for (int h = 0; h < kHold; ++h)
+                held[h] = held_strip(h, kStripsPerBlock) < kStripsPerBlock ? strip : -kInf; /* a strip's own threads hold it */
+            select_top<T>(p, r, l, mask, v, o, held, [](int) { return -kInf; }, kStripsPerBlock, chunk_vecs, chunk_len, top);
         }
     }
 }
@@ -634,22 +619,27 @@ __global__ void __launch_bounds__(kBlock) k_policy_join(const Row p, int chunks,
     const int64_t r = blockIdx.x;
     const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
     const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
+    const int n_strips = p.top > 0 ? chunks * kStripsPerBlock : 0;
+    const float* mine = strips + r * chunks * kStripsPerBlock;
+    /* everything the row needs is asked for at once */
+    float held[kHold];
+    _Pragma("unroll") for (int h = 0; h < kHold; ++h) {
+        const int i = held_strip(h, n_strips);
+        held[h] = i < n_strips ? mine[i] : -kInf;
+    }
     Sum v{-kInf, 0.0f, 0.0f};
     if ((int)threadIdx.x < chunks) {
         const float* q = parts + 3 * (r * chunks + threadIdx.x);
         v = Sum{q[0], q[1], q[2]};
     }
+    const int64_t a = row_action(p, r);
+    const float la = action_logit<T>(p, l, mask, a);
     v = block_merge<kBlock>(p, v, lds);
     const Values o = row_values(p, v);
-    if (threadIdx.x == 0) {
-        const int64_t a = row_action(p, r);
-        write_row(p, r, v, o, action_logit<T>(p, l, mask, a), a);
-    }
-    if (p.top > 0) {
-        const float* mine = strips + r * chunks * kBlock;
-        select_top<T, kBlock>(p, r, l, mask, v, o, [&](int i) { return mine[i]; }, chunks * kBlock, chunk_vecs,
-                              (uint32_t)chunk_vecs * kBlock * Kind<T>::kPer, top);
-    }
+    if (threadIdx.x == 0) write_row(p, r, v, o, la, a);
+    if (p.top > 0)
+        select_top<T>(p, r, l, mask, v, o, held, [&](int i) { return mine[i]; }, n_strips, chunk_vecs,
+                      (uint32_t)chunk_vecs * kBlock * Kind<T>::kPer, top);
 }
 
 /* gradient of one vector */
@@ -883,7 +873,7 @@ size_t workspace_bytes(const mzs_policy_args& a, int per) {
     if (a.rows == 0 || a.n_actions <= kLanesMost) return 0;
     const Cut c = cut_row(a.rows, a.n_actions, per, true);
     if (c.chunks == 1) return 0;
-    return sizeof(float) * (size_t)a.rows * c.chunks * (3 + (a.top > 0 ? kBlock : 0));
+    return sizeof(float) * (size_t)a.rows * c.chunks * (3 + (a.top > 0 ? kStripsPerBlock : 0));
 }
 
 int run(const mzs_policy_args* a, void* stream, bool forward, bool grad) {
