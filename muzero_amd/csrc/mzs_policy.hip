@@ -50,7 +50,9 @@ struct Kind<float> {
     static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
     static __device__ __forceinline__ float get(const w4& v, int j) { return __uint_as_float(v[j]); }
     static __device__ __forceinline__ void set(w4& v, int j, float x) { v[j] = __float_as_uint(x); }
-    static __device__ __forceinline__ void keep(w4& v, int j, bool k) { v[j] = k ? v[j] : kNone; }
+    static __device__ __forceinline__ void keep(w4& v, const uint32_t* m) { /* a byte of m for each */
+        _Pragma("unroll") for (int j = 0; j < 4; ++j) v[j] = (m[0] >> (8 * j)) & 0xffu ? v[j] : kNone;
+    }
     static __device__ __forceinline__ w4 pack(const float* x) {
         return w4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
     }
@@ -58,8 +60,17 @@ struct Kind<float> {
 template <typename T>
 struct Half { /* two to a word */
     static constexpr int kPer = 8;
-    static __device__ __forceinline__ void set_bits(w4& v, int j, uint32_t x) {
-        v[j >> 1] = j & 1 ? (v[j >> 1] & 0xffffu) | (x << 16) : (v[j >> 1] & 0xffff0000u) | x;
+    /* Where a byte of m is 0 the element becomes `none`: the byte's top bit is set if it is not 0, v_perm_b32 spreads two of those bits
+     * over the halves of a word (selectors 8 .. 11: the signs of the four halves of its operands), v_bfi_b32 picks: two operations an
+     * element, where a comparison and a selection each would be four. */
+    template <uint32_t none>
+    static __device__ __forceinline__ void keep_halves(w4& v, const uint32_t* m) {
+        _Pragma("unroll") for (int h = 0; h < 2; ++h) {
+            const uint32_t t = ((m[h] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | m[h], up = t << 8;
+            const uint32_t first = __builtin_amdgcn_perm(up, t, 0x08080a0au), second = __builtin_amdgcn_perm(up, t, 0x09090b0bu);
+            v[2 * h] = (v[2 * h] & first) | (none * 0x10001u & ~first);
+            v[2 * h + 1] = (v[2 * h + 1] & second) | (none * 0x10001u & ~second);
+        }
     }
 };
 template <>
@@ -72,7 +83,7 @@ struct Kind<__bf16> : Half<__bf16> {
     static __device__ __forceinline__ float get(const w4& v, int j) {
         return __uint_as_float(j & 1 ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16);
     }
-    static __device__ __forceinline__ void keep(w4& v, int j, bool k) { if (!k) set_bits(v, j, kNone); }
+    static __device__ __forceinline__ void keep(w4& v, const uint32_t* m) { keep_halves<kNone>(v, m); }
     static __device__ __forceinline__ w4 pack(const float* x) { /* v_cvt_pk_bf16_f32: nearest even, NaN kept */
         w4 v;
         _Pragma("unroll") for (int i = 0; i < 4; ++i)
@@ -88,7 +99,7 @@ struct Kind<_Float16> : Half<_Float16> {
     static __device__ __forceinline__ float get(const w4& v, int j) {
         return (float)__builtin_bit_cast(_Float16, (uint16_t)(j & 1 ? v[j >> 1] >> 16 : v[j >> 1]));
     }
-    static __device__ __forceinline__ void keep(w4& v, int j, bool k) { if (!k) set_bits(v, j, kNone); }
+    static __device__ __forceinline__ void keep(w4& v, const uint32_t* m) { keep_halves<kNone>(v, m); }
     static __device__ __forceinline__ w4 pack(const float* x) {
         w4 v;
         _Pragma("unroll") for (int i = 0; i < 4; ++i)
@@ -109,26 +120,33 @@ __device__ __forceinline__ w4 move_down(const w4& x, uint32_t by) {
     return w4{(uint32_t)y0, (uint32_t)(y0 >> 32), (uint32_t)y1, (uint32_t)(y1 >> 32)};
 }
 
-/* N vectors of a row from element i on, `stride` elements apart; what the mask forbids and what lies behind the row's end is -inf.  Every
- * lane loads inside the row (n >= kPer): a vector that the end cuts is loaded from n - kPer on and moved down, so that the
- * loads go out back to back whatever the row's end.  l and mask are uniform over the block: scalar base, 32-bit byte offset. */
+/* N vectors of a row from element i on, `stride` elements apart, as they are in memory.  Every lane loads inside the row (n >= kPer): a
+ * vector that the row's end cuts is loaded from n - kPer on, so that the loads go out back to back whatever the end.  l is uniform
+ * over the block: scalar base, 32-bit byte offset. */
+template <typename T, int N>
+__device__ __forceinline__ void load_raw(const T* __restrict__ l, uint32_t i, uint32_t stride, uint32_t n, w4* x) {
+    _Pragma("unroll") for (int u = 0; u < N; ++u) {
+        const uint32_t at = min(i + u * stride, n - Kind<T>::kPer);
+        x[u] = *reinterpret_cast<const w4_any*>(reinterpret_cast<const char*>(l) + (uint32_t)(at * sizeof(T)));
+    }
+}
+/* what the mask forbids and what lies behind the row's end becomes -inf; cut vectors move down to where they belong */
+template <typename T, int N>
+__device__ __forceinline__ void dress(const uint8_t* __restrict__ mask, uint32_t i, uint32_t stride, uint32_t n, w4* x) {
+    constexpr int kPer = Kind<T>::kPer;
+    if (mask) {
+        uint32_t m[N][kPer / 4];
+        _Pragma("unroll") for (int u = 0; u < N; ++u) __builtin_memcpy(m[u], mask + min(i + u * stride, n - kPer), kPer);
+        _Pragma("unroll") for (int u = 0; u < N; ++u) Kind<T>::keep(x[u], m[u]);
+    }
+    _Pragma("unroll") for (int u = 0; u < N; ++u)
+        if (i + u * stride > n - kPer) x[u] = move_down<T>(x[u], i + u * stride - (n - kPer));
+}
 template <typename T, int N>
 __device__ __forceinline__ void load_vecs(const T* __restrict__ l, const uint8_t* __restrict__ mask, uint32_t i, uint32_t stride, uint32_t n,
                                           w4* x) {
-    constexpr int kPer = Kind<T>::kPer;
-    uint32_t at[N];
-    _Pragma("unroll") for (int u = 0; u < N; ++u) {
-        at[u] = min(i + u * stride, n - kPer);
-        x[u] = *reinterpret_cast<const w4_any*>(reinterpret_cast<const char*>(l) + (uint32_t)(at[u] * sizeof(T)));
-    }
-    if (mask) {
-        uint32_t m[N][kPer / 4];
-        _Pragma("unroll") for (int u = 0; u < N; ++u) __builtin_memcpy(m[u], mask + at[u], kPer);
-        _Pragma("unroll") for (int u = 0; u < N; ++u)
-            _Pragma("unroll") for (int j = 0; j < kPer; ++j) Kind<T>::keep(x[u], j, (m[u][j / 4] >> (8 * (j % 4))) & 0xffu);
-    }
-    _Pragma("unroll") for (int u = 0; u < N; ++u)
-        if (i + u * stride > n - kPer) x[u] = move_down<T>(x[u], i + u * stride - at[u]);
+    load_raw<T, N>(l, i, stride, n, x);
+    dress<T, N>(mask, i, stride, n, x);
 }
 template <typename T>
 __device__ __forceinline__ w4 load_vec(const T* __restrict__ l, const uint8_t* __restrict__ mask, uint32_t i, uint32_t n) {
@@ -136,19 +154,9 @@ __device__ __forceinline__ w4 load_vec(const T* __restrict__ l, const uint8_t* _
     load_vecs<T, 1>(l, mask, i, 0, n, &x);
     return x;
 }
-/* the elements of v that the row has go to [i, i + kPer) */
 template <typename T>
-__device__ __forceinline__ void store_vec(T* __restrict__ g, uint32_t i, uint32_t n, const w4& v) {
-    constexpr int kPer = Kind<T>::kPer;
-    if (i + kPer <= n) {
-        *reinterpret_cast<w4_any*>(reinterpret_cast<char*>(g) + (uint32_t)(i * sizeof(T))) = v;
-    } else if (i < n) { /* one thread's: short code before fast code */
-        const uint64_t w0 = v[0] | ((uint64_t)v[1] << 32), w1 = v[2] | ((uint64_t)v[3] << 32);
-        _Pragma("clang loop unroll(disable)") for (uint32_t j = 0; i + j < n; ++j) {
-            const uint32_t bit = j * 8 * sizeof(T), bits = (uint32_t)((bit < 64u ? w0 : w1) >> (bit & 63u));
-            __builtin_memcpy(g + i + j, &bits, sizeof(T));
-        }
-    }
+__device__ __forceinline__ void store_vec(T* __restrict__ g, uint32_t i, const w4& v) {
+    *reinterpret_cast<w4_any*>(reinterpret_cast<char*>(g) + (uint32_t)(i * sizeof(T))) = v;
 }
 
 /* one part of a row: its largest logit, and s and t relative to it */
@@ -203,6 +211,11 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return lanes_reduce<G>(v, [](float a, float b) { return a + b; });
 }
 
+/* c * big overflows, or its products lose the differences: such rows (the type's lowest values as a mask, all of them; 1e30 and
+ * more) take their exponents as c (l_i - big) */
+constexpr float kHuge = 1e30f;
+__device__ __forceinline__ bool is_huge(const Row& p, float big) { return !(fabsf(p.c * big) < kHuge); }
+
 /* exponent of 2 for a logit x beside the row's largest one; finite, so that 0 * it is 0 */
 __device__ __forceinline__ float exponent_of(const Row& p, float x, float big) { return fmaxf(p.c * (x - big), kLow); }
 /* 2^d; a NaN logit (which fmaxf turned into kLow) stays one */
@@ -240,26 +253,33 @@ __device__ __forceinline__ void write_top(const Row& p, int64_t r, int k, uint64
     p.top_log_prob[r * p.top + k] = key ? p.scale * (key_value(key) - v.big) - o.log_total : -kInf;
 }
 
-/* What the gradient of a row needs: grad_i = e_i (base + slope d_i), + at_action where i is the action. */
+/* What the gradient of a row needs: grad_i = 2^(c l_i - m) (base + slope (c l_i - m)), + at_action where i is the action. */
 struct Slope {
-    float big, base, slope, at_action;
+    float big, m, base, slope, at_action;
     bool empty;
 };
 __device__ __forceinline__ Slope row_slope(const Row& p, int64_t r, int64_t a, const Sum& v, float entropy, float log2_s) {
     const float ga = a < 0 || !p.grad_log_prob ? 0.0f : a >= p.n ? __builtin_nanf("") : p.grad_log_prob[r];
     const float gh = p.grad_entropy ? p.grad_entropy[r] : 0.0f, gz = p.grad_log_z ? p.grad_log_z[r] : 0.0f;
-    const float f = p.scale / v.s; /* log p_i = ln 2 (d_i - log2 s) */
     Slope q;
     q.big = v.big;
-    q.base = f * (gz - ga - gh * (entropy - kLn2 * log2_s));
+    q.m = p.c * v.big;
+    const float delta = is_huge(p, v.big) ? 0.0f : fmaf(p.c, v.big, -q.m);
+    const float f = p.scale / v.s * __builtin_amdgcn_exp2f(-delta); /* log p_i = ln 2 (c l_i - m - delta - log2 s) */
+    q.base = f * (gz - ga - gh * (entropy - kLn2 * (log2_s + delta)));
     q.slope = f * (-gh * kLn2);
     q.at_action = p.scale * ga;
     q.empty = v.s == 0.0f;
     return q;
 }
+/* any logit, whatever the row (a huge one has m = 0 in effect: its exponents are differences of logits) */
 __device__ __forceinline__ float slope_at(const Row& p, const Slope& q, float x) {
-    const float d = exponent_of(p, x, q.big);
+    const float d = is_huge(p, q.big) ? exponent_of(p, x, q.big) : fmaxf(fmaf(p.c, x, -q.m), kLow);
     return power_of(d, x) * (q.base + q.slope * d);
+}
+/* whether the short form of the gradient does for the row: c l_i - m as one fma, no element needs a look of its own */
+__device__ __forceinline__ bool is_plain(const Row& p, const Slope& q) {
+    return !q.empty && !is_huge(p, q.big) && fabsf(q.base) < kInf && fabsf(q.slope) < kInf;
 }
 
 /* ------------------------------------------------------------------ narrow rows
@@ -342,33 +362,29 @@ __global__ void __launch_bounds__(kBlock) k_policy_lanes(const Row p) {
 /* ------------------------------------------------------------------ wide rows
  * A block walks a chunk of a row: thread t takes the 16-byte vectors t, t + kBlock, ... of it. */
 
-/* largest value over the block, in every thread.  lds: a float a wave */
-template <int kThreads>
-__device__ __forceinline__ float block_max(float v, float* lds) {
-    v = lanes_max<64>(v);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    _Pragma("unroll") for (int w = 0; w < kThreads / 64; ++w) v = fmaxf(v, lds[w]);
-    return v;
-}
-/* s and t, relative to the block's maximum, summed over the block, in every thread.  lds: two floats a wave, others than block_max's */
-template <int kThreads>
-__device__ __forceinline__ Sum block_sum(float big, float s, float t, float* lds) {
-    constexpr int kWaves = kThreads / 64;
-    s = lanes_sum<64>(s), t = lanes_sum<64>(t);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s, lds[kWaves + (threadIdx.x >> 6)] = t;
-    __syncthreads();
-    Sum o{big, 0.0f, 0.0f};
-    _Pragma("unroll") for (int w = 0; w < kWaves; ++w) o.s += lds[w], o.t += lds[kWaves + w];
+/* A team of threads works on a row: a wave, or a whole block.  Merges every thread's part; all threads return the same bits.
+ * lds: three floats a wave (a block's team) */
+template <int kTeam>
+__device__ __forceinline__ Sum team_merge(const Row& p, Sum v, float* lds) {
+    constexpr int kWaves = kTeam / 64;
+    const int wave = threadIdx.x >> 6;
+    const bool first = (threadIdx.x & 63) == 0;
+    float big = lanes_max<64>(v.big);
+    if constexpr (kWaves > 1) {
+        if (first) lds[wave] = big;
+        __syncthreads();
+        _Pragma("unroll") for (int w = 0; w < kWaves; ++w) big = fmaxf(big, lds[w]);
+    }
+    const float d = v.big == big ? 0.0f : fmaxf(p.c * (v.big - big), kLow), f = __builtin_amdgcn_exp2f(d);
+    Sum o{big, lanes_sum<64>(f * v.s), lanes_sum<64>(f * (v.t + d * v.s))};
+    if constexpr (kWaves > 1) {
+        if (first) lds[kWaves + wave] = o.s, lds[2 * kWaves + wave] = o.t;
+        __syncthreads();
+        o.s = o.t = 0.0f;
+        _Pragma("unroll") for (int w = 0; w < kWaves; ++w) o.s += lds[kWaves + w], o.t += lds[2 * kWaves + w];
+    }
     if (big == kInf) o.s = __builtin_nanf("");
     return o;
-}
-/* merges every thread's part; all threads return the whole.  lds: three floats a wave */
-template <int kThreads>
-__device__ __forceinline__ Sum block_merge(const Row& p, Sum v, float* lds) {
-    const float big = block_max<kThreads>(v.big, lds);
-    const float d = v.big == big ? 0.0f : fmaxf(p.c * (v.big - big), kLow), f = __builtin_amdgcn_exp2f(d);
-    return block_sum<kThreads>(big, f * v.s, f * (v.t + d * v.s), lds + kThreads / 64);
 }
 
 constexpr int kAhead = 4; /* vectors a thread has in flight */
@@ -383,26 +399,44 @@ __device__ __forceinline__ float max_vecs(const w4* v, float big) {
         _Pragma("unroll") for (int j = 0; j < Kind<T>::kPer; ++j) big = fmaxf(big, Kind<T>::get(v[u], j));
     return big;
 }
-/* adds the exponentials relative to `ref`, a finite number (or one whose row is NaN anyway) that no logit exceeds */
+/* A thread's running sum over the vectors of a wide row, relative to m = c * big held within +-kHuge: the exponent is one fma, c l_i - m
+ * with a single rounding, and what m lost to its own rounding is put right once at the end.  Where m was held, nothing is
+ * allowed yet (all exponentials are 0) or the row is huge: then the chunk is summed again by sum_slowly. */
+struct Running {
+    float big, m, s, t;
+};
+__device__ __forceinline__ Running running_start() { return Running{-kInf, -kHuge, 0.0f, 0.0f}; }
+
+/* takes N vectors: their maximum first, one rescaling, then the exponentials */
 template <typename T, int N>
-__device__ __forceinline__ void sum_vecs(const Row& p, const w4* v, float ref, float& s, float& t) {
+__device__ __forceinline__ void take_vecs(const Row& p, const w4* v, Running& sum) {
+    const float big = max_vecs<T, N>(v, sum.big), m = __builtin_amdgcn_fmed3f(p.c * big, -kHuge, kHuge);
+    const float shift = fmaxf(sum.m - m, kLow), f = __builtin_amdgcn_exp2f(shift);
+    float s = f * sum.s, t = f * (sum.t + shift * sum.s);
     _Pragma("unroll") for (int u = 0; u < N; ++u)
         _Pragma("unroll") for (int j = 0; j < Kind<T>::kPer; ++j) {
-            const float d = p.c * (Kind<T>::get(v[u], j) - ref), e = __builtin_amdgcn_exp2f(d);
+            const float d = fmaf(p.c, Kind<T>::get(v[u], j), -m), e = __builtin_amdgcn_exp2f(d);
             s += e, t = fmaf(e, fmaxf(d, kLow), t);
         }
+    sum = Running{big, m, s, t};
 }
-/* nothing allowed: relative to 0 every exponential is 0 (or NaN) */
-__device__ __forceinline__ float reference(float big) { return big == -kInf ? 0.0f : big; }
-
-/* takes N vectors into a thread's running sum: their maximum first, one rescaling, then the exponentials */
-template <typename T, int N>
-__device__ __forceinline__ void take_vecs(const Row& p, const w4* v, Sum& sum) {
-    const float big = max_vecs<T, N>(v, sum.big);
-    const float shift = sum.big == big ? 0.0f : fmaxf(p.c * (sum.big - big), kLow), f = __builtin_amdgcn_exp2f(shift);
-    float s = f * sum.s, t = f * (sum.t + shift * sum.s);
-    sum_vecs<T, N>(p, v, reference(big), s, t);
-    sum = Sum{big, s, t};
+/* the same relative to big itself */
+__device__ __forceinline__ Sum running_end(const Row& p, const Running& v) {
+    const float delta = is_huge(p, v.big) ? 0.0f : fmaf(p.c, v.big, -v.m), f = __builtin_amdgcn_exp2f(-delta);
+    return Sum{v.big, f * v.s, f * (v.t - delta * v.s)};
+}
+/* this thread's vectors i, i + stride, ... of a row whose largest logit `big` is huge */
+template <typename T>
+__device__ Sum sum_slowly(const Row& p, const T* l, const uint8_t* mask, uint32_t i, uint32_t stride, uint32_t end, uint32_t n, float big) {
+    Sum v{big, 0.0f, 0.0f};
+    for (; i < end && i < n; i += stride) {
+        const w4 x = load_vec<T>(l, mask, i, n);
+        _Pragma("unroll") for (int j = 0; j < Kind<T>::kPer; ++j) {
+            const float y = Kind<T>::get(x, j), d = exponent_of(p, y, big), e = power_of(d, y);
+            v.s += e, v.t = fmaf(e, d, v.t);
+        }
+    }
+    return v;
 }
 
 constexpr int kStrips = 512; /* strips that can hold alternatives              */
@@ -577,19 +611,32 @@ __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks
     const uint32_t chunk_len = (uint32_t)chunk_vecs * kBlock * kPer, from = chunk * chunk_len + threadIdx.x * kPer;
     const int64_t a = kSplit ? -1 : row_action(p, r); /* asked for early: nothing waits for it behind the sums */
     const float la = kSplit ? 0.0f : action_logit<T>(p, l, mask, a);
-    Sum v{-kInf, 0.0f, 0.0f};
-    int j = 0;
-    for (; j + kAhead <= chunk_vecs; j += kAhead) {
-        w4 x[kAhead];
-        load_vecs<T, kAhead>(l, mask, from + (uint32_t)j * kBlock * kPer, kBlock * kPer, n, x);
-        take_vecs<T, kAhead>(p, x, v);
+    Running sum = running_start();
+    constexpr uint32_t kStride = kBlock * kPer;
+    const int groups = chunk_vecs / kAhead; /* the next group is on its way while one is summed */
+    w4 x[kAhead], y[kAhead];
+    const auto load = [&](int g, w4* v) { if (g < groups) load_raw<T, kAhead>(l, from + (uint32_t)g * kAhead * kStride, kStride, n, v); };
+    const auto take = [&](int g, w4* v) {
+        dress<T, kAhead>(mask, from + (uint32_t)g * kAhead * kStride, kStride, n, v);
+        take_vecs<T, kAhead>(p, v, sum);
+    };
+    load(0, x);
+    for (int g = 0; g < groups; g += 2) {
+        load(g + 1, y);
+        take(g, x);
+        load(g + 2, x);
+        if (g + 1 < groups) take(g + 1, y);
     }
-    for (; j < chunk_vecs; ++j) {
-        w4 x = load_vec<T>(l, mask, from + (uint32_t)j * kBlock * kPer, n);
-        take_vecs<T, 1>(p, &x, v);
+    for (int j = groups * kAhead; j < chunk_vecs; ++j) {
+        w4 z = load_vec<T>(l, mask, from + (uint32_t)j * kStride, n);
+        take_vecs<T, 1>(p, &z, sum);
     }
-    const float strip = lanes_max<kStripLanes>(v.big);
-    v = block_merge<kBlock>(p, v, lds);
+    const float strip = lanes_max<kStripLanes>(sum.big);
+    Sum v = team_merge<kBlock>(p, running_end(p, sum), lds);
+    if (is_huge(p, v.big) && fabsf(v.big) < kInf) {
+        __syncthreads();
+        v = team_merge<kBlock>(p, sum_slowly<T>(p, l, mask, from, kBlock * kPer, (chunk + 1) * chunk_len, n, v.big), lds);
+    }
     if constexpr (kSplit) {
         if (p.top > 0 && threadIdx.x % kStripLanes == 0)
             strips[(int64_t)blockIdx.x * kStripsPerBlock + threadIdx.x / kStripLanes] = strip;
@@ -634,7 +681,7 @@ __global__ void __launch_bounds__(kBlock) k_policy_join(const Row p, int chunks,
     }
     const int64_t a = row_action(p, r);
     const float la = action_logit<T>(p, l, mask, a);
-    v = block_merge<kBlock>(p, v, lds);
+    v = team_merge<kBlock>(p, v, lds);
     const Values o = row_values(p, v);
     if (threadIdx.x == 0) write_row(p, r, v, o, la, a);
     if (p.top > 0)
@@ -642,21 +689,39 @@ __global__ void __launch_bounds__(kBlock) k_policy_join(const Row p, int chunks,
                       (uint32_t)chunk_vecs * kBlock * Kind<T>::kPer, top);
 }
 
-/* gradient of one vector */
+/* v_mul_legacy_f32: a product in which 0 times anything is 0 */
+__device__ float mul_zero_wins(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+
+/* Gradient of one vector of a plain row, without the action's own part.  The product is the one in which 0 times anything is 0: an
+ * exponential of 0 comes with an exponent of -inf where the logit is -inf. */
 template <typename T>
-__device__ __forceinline__ w4 slope_vec(const Row& p, const Slope& q, const w4& x, uint32_t i, uint32_t action) {
+__device__ __forceinline__ w4 slope_vec(const Row& p, const Slope& q, const w4& x) {
     constexpr int kPer = Kind<T>::kPer;
     float y[kPer];
     _Pragma("unroll") for (int j = 0; j < kPer; ++j) {
-        const float l = Kind<T>::get(x, j);
-        const float d0 = p.c * (l - q.big), e = __builtin_amdgcn_exp2f(d0);
-        y[j] = e * fmaf(q.slope, fmaxf(d0, kLow), q.base);
+        const float d = fmaf(p.c, Kind<T>::get(x, j), -q.m);
+        y[j] = mul_zero_wins(__builtin_amdgcn_exp2f(d), fmaf(q.slope, d, q.base));
     }
-    if (action - i < kPer)
-        _Pragma("unroll") for (int j = 0; j < kPer; ++j) if (i + j == action && Kind<T>::get(x, j) != -kInf) y[j] += q.at_action;
-    if (!(fabsf(q.base) < kInf)) /* NaN or infinite coefficients: elements that are not allowed stay 0 all the same */
-        _Pragma("unroll") for (int j = 0; j < kPer; ++j) if (Kind<T>::get(x, j) == -kInf) y[j] = 0.0f;
     return Kind<T>::pack(y);
+}
+/* elements [from, to) of a row one by one: rows that are not plain, and the last few of those that are */
+template <typename T, int kTeam>
+__device__ void slope_slowly(const Row& p, const Slope& q, const T* l, const uint8_t* mask, T* out, uint32_t from, uint32_t to,
+                                          uint32_t action) {
+    for (uint32_t i = from + threadIdx.x % kTeam; i < to; i += kTeam) {
+        const float x = mask && !mask[i] ? -kInf : Kind<T>::load(l + i);
+        float y = 0.0f;
+        if (!q.empty && x != -kInf) {
+            y = slope_at(p, q, x);
+            if (i == action) y += q.at_action;
+        }
+        Kind<T>::store(out + i, y);
+    }
+}
+/* the action's element, over what its vector's store put there: by the same thread, behind it */
+template <typename T>
+__device__ __forceinline__ void store_action(const Row& p, const Slope& q, float la, T* out, uint32_t action) {
+    if (la != -kInf) Kind<T>::store(out + action, slope_at(p, q, la) + q.at_action);
 }
 
 /* gradient of chunks from the rows' stored statistics */
@@ -669,10 +734,16 @@ __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks
     const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
     T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
     const int64_t a = row_action(p, r);
+    const float la = action_logit<T>(p, l, mask, a);
     const Sum v{p.row_stats[2 * r], p.row_stats[2 * r + 1], 0.0f};
     const Slope q = row_slope(p, r, a, v, p.entropy[r], log2f(v.s));
-    const uint32_t n = (uint32_t)p.n, action = a >= 0 && a < p.n ? (uint32_t)a : ~0u;
-    const uint32_t from = ((uint32_t)chunk * chunk_vecs * kBlock + threadIdx.x) * kPer;
+    const uint32_t n = (uint32_t)p.n, action = a >= 0 && a < p.n ? (uint32_t)a : ~0u, whole = n - n % kPer;
+    const uint32_t first = (uint32_t)chunk * chunk_vecs * kBlock * kPer, end = min(first + (uint32_t)chunk_vecs * kBlock * kPer, n);
+    if (!is_plain(p, q)) {
+        slope_slowly<T, kBlock>(p, q, l, mask, out, first, end, action);
+        return;
+    }
+    const uint32_t from = first + threadIdx.x * kPer;
     int j = 0;
     for (; j + kAhead <= chunk_vecs; j += kAhead) {
         w4 x[kAhead];
@@ -680,51 +751,71 @@ __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks
         load_vecs<T, kAhead>(l, mask, i, kBlock * kPer, n, x);
         _Pragma("unroll") for (int u = 0; u < kAhead; ++u) {
             const uint32_t at = i + u * kBlock * kPer;
-            store_vec<T>(out, at, n, q.empty ? w4{0, 0, 0, 0} : slope_vec<T>(p, q, x[u], at, action));
+            if (at < whole) store_vec<T>(out, at, slope_vec<T>(p, q, x[u]));
         }
     }
     for (; j < chunk_vecs; ++j) {
         const uint32_t i = from + (uint32_t)j * kBlock * kPer;
         const w4 x = load_vec<T>(l, mask, i, n);
-        store_vec<T>(out, i, n, q.empty ? w4{0, 0, 0, 0} : slope_vec<T>(p, q, x, i, action));
+        if (i < whole) store_vec<T>(out, i, slope_vec<T>(p, q, x));
     }
+    if (end == n) slope_slowly<T, kBlock>(p, q, l, mask, out, whole, n, action);
+    if (action >= first && action < min(end, whole) && (action - first) / kPer % kBlock == threadIdx.x) store_action<T>(p, q, la, out, action);
 }
 
-/* Forward and gradient of a row that a block holds in registers (V 16-byte vectors a thread): one read and one write of memory.  Without
- * alternatives: their search would hold its registers on top of the row's. */
-template <typename T, int kThreads, int V>
-__global__ void __launch_bounds__(kThreads, 4) k_policy_train(const Row p) {
+/* A row that its team holds in registers (V 16-byte vectors a thread): one read, and with kGrad one write, of memory.  A wave takes rows of
+ * up to 16 vectors a thread, four rows to a block and no barrier; a block of 512 threads wider ones, two blocks to a CU (at most 128
+ * registers a thread), one block a row: blocks that start when others end keep loads, sums and stores of different rows in
+ * flight, where blocks that walk the rows in step (two a CU, loading the next row into the registers just stored) took 292 us
+ * instead of 269 for 4096 x 81920 bf16.  Without alternatives: their search would hold its registers on top of the row's. */
+template <typename T, int kTeam, int V, bool kGrad>
+__global__ void __launch_bounds__(kTeam == 64 ? kBlock : kTeam, kTeam == 64 ? 1 : 4) k_policy_row(const Row p) {
     constexpr int kPer = Kind<T>::kPer;
-    __shared__ float lds[3 * (kThreads / 64)];
-    const int64_t r = blockIdx.x;
+    constexpr uint32_t kStride = kTeam * kPer;
+    constexpr int kGroups = V / kAhead, kRest = V % kAhead;
+    __shared__ float lds[kTeam == 64 ? 1 : 3 * (kTeam / 64)];
+    const int64_t r = kTeam == 64 ? (int64_t)blockIdx.x * (kBlock / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+    if (r >= p.rows) return; /* a whole wave */
+    const uint32_t n = (uint32_t)p.n, lane = threadIdx.x % kTeam;
+    uint32_t from = lane * kPer;
     const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
     const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
-    const uint32_t n = (uint32_t)p.n;
-    uint32_t from = threadIdx.x * kPer;
     w4 x[V];
-    constexpr int kGroups = V / kAhead;
-    _Pragma("unroll") for (int j = 0; j < kGroups; ++j)
-        load_vecs<T, kAhead>(l, mask, from + j * kAhead * kThreads * kPer, kThreads * kPer, n, x + j * kAhead);
-    if constexpr (V % kAhead != 0)
-        load_vecs<T, V % kAhead>(l, mask, from + kGroups * kAhead * kThreads * kPer, kThreads * kPer, n, x + kGroups * kAhead);
+    load_raw<T, V>(l, from, kStride, n, x);
     const int64_t a = row_action(p, r);
     const float la = action_logit<T>(p, l, mask, a); /* before the gradient may overwrite it */
-    _Pragma("unroll") for (int j = 0; j < V; ++j) unpack_here(x[j]);
-    const float big = block_max<kThreads>(max_vecs<T, V>(x, -kInf), lds);
-    _Pragma("unroll") for (int j = 0; j < V; ++j) unpack_here(x[j]);
-    float s = 0.0f, t = 0.0f;
-    sum_vecs<T, V>(p, x, reference(big), s, t);
-    const Sum v = block_sum<kThreads>(big, s, t, lds + kThreads / 64);
+    Running sum = running_start();
+    _Pragma("unroll") for (int j = 0; j < kGroups; ++j) {
+        dress<T, kAhead>(mask, from + j * kAhead * kStride, kStride, n, x + j * kAhead);
+        take_vecs<T, kAhead>(p, x + j * kAhead, sum);
+    }
+    if constexpr (kRest != 0) {
+        dress<T, kRest>(mask, from + kGroups * kAhead * kStride, kStride, n, x + kGroups * kAhead);
+        take_vecs<T, kRest>(p, x + kGroups * kAhead, sum);
+    }
+    Sum v = team_merge<kTeam>(p, running_end(p, sum), lds);
+    if (is_huge(p, v.big) && fabsf(v.big) < kInf) {
+        if (kTeam > 64) __syncthreads();
+        v = team_merge<kTeam>(p, sum_slowly<T>(p, l, mask, from, kStride, n, n, v.big), lds);
+    }
     const Values o = row_values(p, v);
-    if (threadIdx.x == 0) write_row(p, r, v, o, la, a);
-    const Slope q = row_slope(p, r, a, v, o.entropy, o.log2_s);
-    T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
-    const uint32_t action = a >= 0 && a < p.n ? (uint32_t)a : ~0u;
-    asm volatile("" : "+v"(from)); /* the places are worked out anew, not kept since the loads */
-    _Pragma("unroll") for (int j = 0; j < V; ++j) {
-        const uint32_t i = from + j * kThreads * kPer;
-        unpack_here(x[j]);
-        store_vec<T>(out, i, n, q.empty ? w4{0, 0, 0, 0} : slope_vec<T>(p, q, x[j], i, action));
+    if (lane == 0) write_row(p, r, v, o, la, a);
+    if constexpr (kGrad) {
+        const Slope q = row_slope(p, r, a, v, o.entropy, o.log2_s);
+        T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
+        const uint32_t action = a >= 0 && a < p.n ? (uint32_t)a : ~0u, whole = n - n % kPer;
+        if (!is_plain(p, q)) {
+            slope_slowly<T, kTeam>(p, q, l, mask, out, 0, n, action);
+            return;
+        }
+        asm volatile("" : "+v"(from)); /* the places are worked out anew, not kept since the loads */
+        _Pragma("unroll") for (int j = 0; j < V; ++j) {
+            const uint32_t i = from + j * kStride;
+            unpack_here(x[j]);
+            if (i < whole) store_vec<T>(out, i, slope_vec<T>(p, q, x[j]));
+        }
+        slope_slowly<T, kTeam>(p, q, l, mask, out, whole, n, action);
+        if (action < whole && action / kPer % kTeam == lane) store_action<T>(p, q, la, out, action);
     }
 }
 
@@ -779,6 +870,7 @@ Cut cut_row(int64_t rows, int64_t n, int per, bool join) {
     if (chunks > all) chunks = all;
     Cut c;
     c.vecs = (int)((all + chunks - 1) / chunks);
+    if (c.vecs > kAhead) c.vecs = (c.vecs + kAhead - 1) / kAhead * kAhead; /* whole groups */
     c.chunks = (int)((all + c.vecs - 1) / c.vecs);
     return c;
 }
@@ -815,22 +907,37 @@ void launch_slope(const Row& p, hipStream_t st) {
     hipLaunchKernelGGL(k_policy_slope<T>, dim3((unsigned)(p.rows * c.chunks)), dim3(kBlock), 0, st, p, c.chunks, c.vecs);
 }
 
-constexpr int kTrainThreads = 512, kTrainVecs = 24;
+/* rows in registers: V vectors a thread of a wave (most16) or of a block of 512 */
+constexpr int kRowThreads = 512, kWaveVecs = 16, kRowVecs = 24;
 template <typename T>
-bool fits_train(int64_t n) { return n <= (int64_t)kTrainThreads * kTrainVecs * Kind<T>::kPer; }
+bool fits_wave(int64_t n) { return n <= (int64_t)64 * kWaveVecs * Kind<T>::kPer; }
 template <typename T>
-void launch_train(const Row& p, hipStream_t st) {
-    const int64_t all = (p.n + (int64_t)kTrainThreads * Kind<T>::kPer - 1) / ((int64_t)kTrainThreads * Kind<T>::kPer);
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.rows), dim3(kTrainThreads), 0, st, p); };
-    if (all <= 1) go(k_policy_train<T, kTrainThreads, 1>);
-    else if (all <= 2) go(k_policy_train<T, kTrainThreads, 2>);
-    else if (all <= 4) go(k_policy_train<T, kTrainThreads, 4>);
-    else if (all <= 8) go(k_policy_train<T, kTrainThreads, 8>);
-    else if (all <= 12) go(k_policy_train<T, kTrainThreads, 12>);
-    else if (all <= 16) go(k_policy_train<T, kTrainThreads, 16>);
-    else if (all <= 20) go(k_policy_train<T, kTrainThreads, 20>);
-    else if (all <= 21) go(k_policy_train<T, kTrainThreads, 21>);
-    else go(k_policy_train<T, kTrainThreads, kTrainVecs>);
+bool fits_block(int64_t n) { return n <= (int64_t)kRowThreads * kRowVecs * Kind<T>::kPer; }
+template <typename T, bool kGrad>
+void launch_wave_row(const Row& p, hipStream_t st) {
+    const int64_t all = (p.n + 64 * Kind<T>::kPer - 1) / (64 * Kind<T>::kPer);
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((p.rows + kBlock / 64 - 1) / (kBlock / 64))), dim3(kBlock), 0, st, p);
+    };
+    if (all <= 4) go(k_policy_row<T, 64, 4, kGrad>);
+    else if (all <= 6) go(k_policy_row<T, 64, 6, kGrad>);
+    else if (all <= 8) go(k_policy_row<T, 64, 8, kGrad>);
+    else if (all <= 12) go(k_policy_row<T, 64, 12, kGrad>);
+    else go(k_policy_row<T, 64, 16, kGrad>);
+}
+template <typename T>
+void launch_block_row(const Row& p, hipStream_t st) {
+    const int64_t all = (p.n + (int64_t)kRowThreads * Kind<T>::kPer - 1) / ((int64_t)kRowThreads * Kind<T>::kPer);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.rows), dim3(kRowThreads), 0, st, p); };
+    if (all <= 3) go(k_policy_row<T, kRowThreads, 3, true>);
+    else if (all <= 4) go(k_policy_row<T, kRowThreads, 4, true>);
+    else if (all <= 6) go(k_policy_row<T, kRowThreads, 6, true>);
+    else if (all <= 8) go(k_policy_row<T, kRowThreads, 8, true>);
+    else if (all <= 12) go(k_policy_row<T, kRowThreads, 12, true>);
+    else if (all <= 16) go(k_policy_row<T, kRowThreads, 16, true>);
+    else if (all <= 20) go(k_policy_row<T, kRowThreads, 20, true>);
+    else if (all <= 21) go(k_policy_row<T, kRowThreads, 21, true>);
+    else go(k_policy_row<T, kRowThreads, kRowVecs, true>);
 }
 
 constexpr int64_t kSlab = 1 << 20; /* rows of a launch: blocks times threads stay below 2^32 */
@@ -860,8 +967,13 @@ void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool for
     }
     for (int64_t r = 0; r < all.rows; r += kSlab) {
         const Row p = rows_from<T>(all, r, all.rows - r < kSlab ? all.rows - r : kSlab);
-        if (forward && grad && p.top == 0 && fits_train<T>(p.n)) {
-            launch_train<T>(p, st);
+        if (forward && p.top == 0 && fits_wave<T>(p.n)) {
+            if (grad) launch_wave_row<T, true>(p, st);
+            else launch_wave_row<T, false>(p, st);
+            continue;
+        }
+        if (forward && grad && p.top == 0 && fits_block<T>(p.n)) {
+            launch_block_row<T>(p, st);
             continue;
         }
         if (forward) launch_forward<T>(p, a, st);
