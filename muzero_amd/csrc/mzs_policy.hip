@@ -362,21 +362,21 @@ __global__ void __launch_bounds__(kBlock) k_policy_lanes(const Row p) {
 /* ------------------------------------------------------------------ wide rows
  * A block walks a chunk of a row: thread t takes the 16-byte vectors t, t + kBlock, ... of it. */
 
-/* A team of threads works on a row: a wave, or a whole block.  Merges every thread's part; all threads return the same bits.
- * lds: three floats a wave (a block's team) */
+/* A team of threads works on a row: some lanes of a wave, a wave, or a whole block.  Merges every thread's part; all threads return the
+ * same bits.  lds: three floats a wave (a block's team) */
 template <int kTeam>
 __device__ __forceinline__ Sum team_merge(const Row& p, Sum v, float* lds) {
-    constexpr int kWaves = kTeam / 64;
+    constexpr int kWaves = kTeam / 64, kLanes = kTeam < 64 ? kTeam : 64;
     const int wave = threadIdx.x >> 6;
     const bool first = (threadIdx.x & 63) == 0;
-    float big = lanes_max<64>(v.big);
+    float big = lanes_max<kLanes>(v.big);
     if constexpr (kWaves > 1) {
         if (first) lds[wave] = big;
         __syncthreads();
         _Pragma("unroll") for (int w = 0; w < kWaves; ++w) big = fmaxf(big, lds[w]);
     }
     const float d = v.big == big ? 0.0f : fmaxf(p.c * (v.big - big), kLow), f = __builtin_amdgcn_exp2f(d);
-    Sum o{big, lanes_sum<64>(f * v.s), lanes_sum<64>(f * (v.t + d * v.s))};
+    Sum o{big, lanes_sum<kLanes>(f * v.s), lanes_sum<kLanes>(f * (v.t + d * v.s))};
     if constexpr (kWaves > 1) {
         if (first) lds[kWaves + wave] = o.s, lds[2 * kWaves + wave] = o.t;
         __syncthreads();
@@ -704,6 +704,15 @@ __device__ __forceinline__ w4 slope_vec(const Row& p, const Slope& q, const w4& 
     }
     return Kind<T>::pack(y);
 }
+/* the elements of a cut vector that the row has */
+template <typename T>
+__device__ __forceinline__ void store_part(T* __restrict__ g, uint32_t i, uint32_t n, const w4& v) {
+    _Pragma("unroll") for (int j = 0; j < Kind<T>::kPer - 1; ++j)
+        if (i + j < n) {
+            const uint32_t bits = sizeof(T) == 4 ? v[j & 3] : v[(j >> 1) & 3] >> (16 * (j & 1));
+            __builtin_memcpy(g + i + j, &bits, sizeof(T));
+        }
+}
 /* elements [from, to) of a row one by one: rows that are not plain, and the last few of those that are */
 template <typename T, int kTeam>
 __device__ void slope_slowly(const Row& p, const Slope& q, const T* l, const uint8_t* mask, T* out, uint32_t from, uint32_t to,
@@ -763,19 +772,22 @@ __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks
     if (action >= first && action < min(end, whole) && (action - first) / kPer % kBlock == threadIdx.x) store_action<T>(p, q, la, out, action);
 }
 
-/* A row that its team holds in registers (V 16-byte vectors a thread): one read, and with kGrad one write, of memory.  A wave takes rows of
- * up to 16 vectors a thread, four rows to a block and no barrier; a block of 512 threads wider ones, two blocks to a CU (at most 128
- * registers a thread), one block a row: blocks that start when others end keep loads, sums and stores of different rows in
- * flight, where blocks that walk the rows in step (two a CU, loading the next row into the registers just stored) took 292 us
- * instead of 269 for 4096 x 81920 bf16.  Without alternatives: their search would hold its registers on top of the row's. */
+/* A row that its team holds in registers (V 16-byte vectors a thread): one read, and with kGrad one write, of memory.  Narrow rows share a
+ * wave (2 to 4 vectors a thread: what a row costs once — logarithms, outputs — is then spread over several rows); a wave takes
+ * rows of up to 16 vectors a thread; a block of 512 threads wider ones, two blocks to a CU (at most 128 registers a thread), one
+ * block a row: blocks that start when others end keep loads, sums and stores of different rows in flight, where blocks that walk the rows
+ * in step (two a CU, loading the next row into the registers just stored) took 292 us instead of 269 for 4096 x 81920 bf16.
+ * Without alternatives: their search would hold its registers on top of the row's. */
 template <typename T, int kTeam, int V, bool kGrad>
-__global__ void __launch_bounds__(kTeam == 64 ? kBlock : kTeam, kTeam == 64 ? 1 : 4) k_policy_row(const Row p) {
+__global__ void __launch_bounds__(kTeam <= 64 ? kBlock : kTeam, kTeam <= 64 ? 1 : 4) k_policy_row(const Row p) {
     constexpr int kPer = Kind<T>::kPer;
     constexpr uint32_t kStride = kTeam * kPer;
     constexpr int kGroups = V / kAhead, kRest = V % kAhead;
-    __shared__ float lds[kTeam == 64 ? 1 : 3 * (kTeam / 64)];
-    const int64_t r = kTeam == 64 ? (int64_t)blockIdx.x * (kBlock / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
-    if (r >= p.rows) return; /* a whole wave */
+    __shared__ float lds[kTeam <= 64 ? 1 : 3 * (kTeam / 64)];
+    const int64_t r = kTeam < 64    ? (int64_t)blockIdx.x * (kBlock / kTeam) + threadIdx.x / kTeam
+                      : kTeam == 64 ? (int64_t)blockIdx.x * (kBlock / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
+                                    : blockIdx.x;
+    if (r >= p.rows) return; /* a whole team, and nothing below reaches past a team */
     const uint32_t n = (uint32_t)p.n, lane = threadIdx.x % kTeam;
     uint32_t from = lane * kPer;
     const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
@@ -813,9 +825,11 @@ __global__ void __launch_bounds__(kTeam == 64 ? kBlock : kTeam, kTeam == 64 ? 1 
             const uint32_t i = from + j * kStride;
             unpack_here(x[j]);
             if (i < whole) store_vec<T>(out, i, slope_vec<T>(p, q, x[j]));
+            else if (kTeam < 64 && i < n) store_part<T>(out, i, n, slope_vec<T>(p, q, x[j]));
         }
-        slope_slowly<T, kTeam>(p, q, l, mask, out, whole, n, action);
-        if (action < whole && action / kPer % kTeam == lane) store_action<T>(p, q, la, out, action);
+        const uint32_t end = kTeam < 64 ? n : whole;
+        if (kTeam >= 64) slope_slowly<T, kTeam>(p, q, l, mask, out, whole, n, action);
+        if (action < end && action / kPer % kTeam == lane) store_action<T>(p, q, la, out, action);
     }
 }
 
@@ -882,10 +896,13 @@ void launch_lanes(const Row& p, hipStream_t st) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(kBlock), 0, st, p);
     };
     if (p.n <= 4) go(k_policy_lanes<T, 1, 4, kForward, kGrad, kTop>, 256);
-    else if (p.n <= 16) go(k_policy_lanes<T, 4, 4, kForward, kGrad, kTop>, 64);
-    else if (p.n <= 64) go(k_policy_lanes<T, 16, 4, kForward, kGrad, kTop>, 16);
-    else if (p.n <= 256) go(k_policy_lanes<T, 16, 16, kForward, kGrad, kTop>, 16);
-    else go(k_policy_lanes<T, 64, 16, kForward, kGrad, kTop>, 4);
+    else if (p.n <= 8) go(k_policy_lanes<T, 1, 8, kForward, kGrad, kTop>, 256);
+    else if constexpr (kTop || !kForward) {
+        if (p.n <= 16) go(k_policy_lanes<T, 4, 4, kForward, kGrad, kTop>, 64);
+        else if (p.n <= 64) go(k_policy_lanes<T, 16, 4, kForward, kGrad, kTop>, 16);
+        else if (p.n <= 256) go(k_policy_lanes<T, 16, 16, kForward, kGrad, kTop>, 16);
+        else go(k_policy_lanes<T, 64, 16, kForward, kGrad, kTop>, 4);
+    }
 }
 
 template <typename T>
@@ -907,23 +924,36 @@ void launch_slope(const Row& p, hipStream_t st) {
     hipLaunchKernelGGL(k_policy_slope<T>, dim3((unsigned)(p.rows * c.chunks)), dim3(kBlock), 0, st, p, c.chunks, c.vecs);
 }
 
-/* rows in registers: V vectors a thread of a wave (most16) or of a block of 512 */
+/* rows in registers: up to kWaveVecs vectors a lane of a wave, kRowVecs a thread of a block of kRowThreads */
 constexpr int kRowThreads = 512, kWaveVecs = 16, kRowVecs = 24;
 template <typename T>
-bool fits_wave(int64_t n) { return n <= (int64_t)64 * kWaveVecs * Kind<T>::kPer; }
+bool fits_wave(int64_t n) { return n >= Kind<T>::kPer && n <= (int64_t)64 * kWaveVecs * Kind<T>::kPer; }
 template <typename T>
 bool fits_block(int64_t n) { return n <= (int64_t)kRowThreads * kRowVecs * Kind<T>::kPer; }
 template <typename T, bool kGrad>
 void launch_wave_row(const Row& p, hipStream_t st) {
-    const int64_t all = (p.n + 64 * Kind<T>::kPer - 1) / (64 * Kind<T>::kPer);
-    const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((p.rows + kBlock / 64 - 1) / (kBlock / 64))), dim3(kBlock), 0, st, p);
+    const int64_t all = (p.n + Kind<T>::kPer - 1) / Kind<T>::kPer;
+    const auto go = [&](auto kernel, int team) {
+        const int64_t per_block = kBlock / team;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((p.rows + per_block - 1) / per_block)), dim3(kBlock), 0, st, p);
     };
-    if (all <= 4) go(k_policy_row<T, 64, 4, kGrad>);
-    else if (all <= 6) go(k_policy_row<T, 64, 6, kGrad>);
-    else if (all <= 8) go(k_policy_row<T, 64, 8, kGrad>);
-    else if (all <= 12) go(k_policy_row<T, 64, 12, kGrad>);
-    else go(k_policy_row<T, 64, 16, kGrad>);
+    if (all <= 2) go(k_policy_row<T, 1, 2, kGrad>, 1);
+    else if (all <= 4) go(k_policy_row<T, 2, 2, kGrad>, 2);
+    else if (all <= 8) go(k_policy_row<T, 4, 2, kGrad>, 4);
+    else if (all <= 12) go(k_policy_row<T, 4, 3, kGrad>, 4);
+    else if (all <= 16) go(k_policy_row<T, 4, 4, kGrad>, 4);
+    else if (all <= 24) go(k_policy_row<T, 8, 3, kGrad>, 8);
+    else if (all <= 32) go(k_policy_row<T, 8, 4, kGrad>, 8);
+    else if (all <= 48) go(k_policy_row<T, 16, 3, kGrad>, 16);
+    else if (all <= 64) go(k_policy_row<T, 16, 4, kGrad>, 16);
+    else if (all <= 96) go(k_policy_row<T, 32, 3, kGrad>, 32);
+    else if (all <= 128) go(k_policy_row<T, 32, 4, kGrad>, 32);
+    else if (all <= 192) go(k_policy_row<T, 64, 3, kGrad>, 64);
+    else if (all <= 256) go(k_policy_row<T, 64, 4, kGrad>, 64);
+    else if (all <= 384) go(k_policy_row<T, 64, 6, kGrad>, 64);
+    else if (all <= 512) go(k_policy_row<T, 64, 8, kGrad>, 64);
+    else if (all <= 768) go(k_policy_row<T, 64, 12, kGrad>, 64);
+    else go(k_policy_row<T, 64, 16, kGrad>, 64);
 }
 template <typename T>
 void launch_block_row(const Row& p, hipStream_t st) {
@@ -956,28 +986,41 @@ Row rows_from(Row p, int64_t r, int64_t rows) {
     p.rows = rows;
     return p;
 }
+/* The ways, by the width of the row (and how a call needs it):
+ *   up to 8 logits              a lane a row, a logit at a time                             k_policy_lanes
+ *   up to 16 vectors a lane     a row in a team's registers, without alternatives           k_policy_row, teams up to a wave
+ *   up to 1024                  alternatives, or the gradient from stored statistics        k_policy_lanes
+ *   up to 24 vectors a thread   forward and gradient of a row in a block's registers        k_policy_row, a block
+ *   beyond                      chunks and their join; the gradient from the statistics     k_policy_chunk, k_policy_join, k_policy_slope */
 template <typename T>
 void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool forward, bool grad) {
-    if (all.n <= kLanesMost) {
-        if (forward && all.top > 0) launch_lanes<T, true, false, true>(all, st);
-        else if (forward && !grad) launch_lanes<T, true, false, false>(all, st);
-        else if (forward) launch_lanes<T, true, true, false>(all, st);
-        if (grad && (!forward || all.top > 0)) launch_lanes<T, false, true, false>(all, st);
-        return;
-    }
-    for (int64_t r = 0; r < all.rows; r += kSlab) {
-        const Row p = rows_from<T>(all, r, all.rows - r < kSlab ? all.rows - r : kSlab);
-        if (forward && p.top == 0 && fits_wave<T>(p.n)) {
-            if (grad) launch_wave_row<T, true>(p, st);
-            else launch_wave_row<T, false>(p, st);
+    const bool wave = fits_wave<T>(all.n) && all.n > 8, lanes = all.n <= kLanesMost;
+    const int64_t slab = wave || lanes ? (int64_t)1 << 24 : kSlab;
+    for (int64_t r = 0; r < all.rows; r += slab) {
+        const Row p = rows_from<T>(all, r, all.rows - r < slab ? all.rows - r : slab);
+        const bool both = forward && grad && p.top == 0;
+        if (both && wave) {
+            launch_wave_row<T, true>(p, st);
             continue;
         }
-        if (forward && grad && p.top == 0 && fits_block<T>(p.n)) {
+        if (both && lanes) {
+            launch_lanes<T, true, true, false>(p, st);
+            continue;
+        }
+        if (both && fits_block<T>(p.n)) {
             launch_block_row<T>(p, st);
             continue;
         }
-        if (forward) launch_forward<T>(p, a, st);
-        if (grad) launch_slope<T>(p, st);
+        if (forward) {
+            if (wave && p.top == 0) launch_wave_row<T, false>(p, st);
+            else if (lanes && p.top > 0) launch_lanes<T, true, false, true>(p, st);
+            else if (lanes) launch_lanes<T, true, false, false>(p, st);
+            else launch_forward<T>(p, a, st);
+        }
+        if (grad) {
+            if (lanes) launch_lanes<T, false, true, false>(p, st);
+            else launch_slope<T>(p, st);
+        }
     }
 }
 
