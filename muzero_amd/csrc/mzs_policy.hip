@@ -13,6 +13,10 @@
 #include <cstdint>
 
 namespace mzs {
+
+/* v_mul_legacy_f32: a product in which 0 times anything is 0 */
+__device__ float mul_zero_wins(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+
 namespace {
 
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -29,6 +33,7 @@ struct Row {
     void* grad_logits;
     int64_t rows, n, logits_stride, mask_stride, grad_stride;
     int32_t action_bytes, top;
+    int32_t values; /* k_policy_row: write the forward values (else the gradient alone is wanted) */
     float scale; /* inverse_temperature              */
     float c;     /* inverse_temperature * log2 e     */
 };
@@ -158,6 +163,12 @@ template <typename T>
 __device__ __forceinline__ void store_vec(T* __restrict__ g, uint32_t i, const w4& v) {
     *reinterpret_cast<w4_any*>(reinterpret_cast<char*>(g) + (uint32_t)(i * sizeof(T))) = v;
 }
+
+/* Wide rows of 2-byte logits at an odd element: their vectors start at the row's second logit, so that every one is 4-byte aligned (a
+ * 16-byte access that is not moves 15 % less a second: 1 GiB read 202 us instead of 169), and the first logit is one
+ * thread's extra. */
+template <typename T>
+__device__ __forceinline__ uint32_t skew_of(const T* l) { return sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(l) & 2) ? 1u : 0u; }
 
 /* one part of a row: its largest logit, and s and t relative to it */
 struct Sum {
@@ -420,15 +431,27 @@ __device__ __forceinline__ void take_vecs(const Row& p, const w4* v, Running& su
         }
     sum = Running{big, m, s, t};
 }
+/* takes one logit */
+__device__ __forceinline__ void take_one(const Row& p, float x, Running& sum) {
+    const float big = fmaxf(sum.big, x), m = __builtin_amdgcn_fmed3f(p.c * big, -kHuge, kHuge);
+    const float shift = fmaxf(sum.m - m, kLow), f = __builtin_amdgcn_exp2f(shift);
+    const float d = fmaf(p.c, x, -m), e = __builtin_amdgcn_exp2f(d);
+    sum = Running{big, m, f * sum.s + e, fmaf(e, fmaxf(d, kLow), f * (sum.t + shift * sum.s))};
+}
 /* the same relative to big itself */
 __device__ __forceinline__ Sum running_end(const Row& p, const Running& v) {
     const float delta = is_huge(p, v.big) ? 0.0f : fmaf(p.c, v.big, -v.m), f = __builtin_amdgcn_exp2f(-delta);
     return Sum{v.big, f * v.s, f * (v.t - delta * v.s)};
 }
-/* this thread's vectors i, i + stride, ... of a row whose largest logit `big` is huge */
+/* this thread's vectors i, i + stride, ... and its extra logit (-inf: none) of a row whose largest logit `big` is huge */
 template <typename T>
-__device__ Sum sum_slowly(const Row& p, const T* l, const uint8_t* mask, uint32_t i, uint32_t stride, uint32_t end, uint32_t n, float big) {
+__device__ Sum sum_slowly(const Row& p, const T* l, const uint8_t* mask, uint32_t i, uint32_t stride, uint32_t end, uint32_t n, float big,
+                          float extra) {
     Sum v{big, 0.0f, 0.0f};
+    {
+        const float d = exponent_of(p, extra, big), e = power_of(d, extra);
+        v.s += e, v.t = fmaf(e, d, v.t);
+    }
     for (; i < end && i < n; i += stride) {
         const w4 x = load_vec<T>(l, mask, i, n);
         _Pragma("unroll") for (int j = 0; j < Kind<T>::kPer; ++j) {
@@ -516,7 +539,8 @@ __device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* m
         if (found <= kStrips) {
             for (uint32_t w = tid; w < found * each; w += kBlock) {
                 const uint32_t strip = sh.strips[w / each], lane = w % kStripLanes, j = w % each / kStripLanes;
-                const uint32_t i = strip / kStripsPerBlock * chunk_len + (j * kBlock + strip % kStripsPerBlock * kStripLanes + lane) * kPer;
+                const uint32_t i =
+                    skew_of(l) + strip / kStripsPerBlock * chunk_len + (j * kBlock + strip % kStripsPerBlock * kStripLanes + lane) * kPer;
                 if (i >= n) continue;
                 const w4 x = load_vec<T>(l, mask, i, n);
                 _Pragma("unroll") for (int q = 0; q < kPer; ++q) {
@@ -525,6 +549,13 @@ __device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* m
                         const uint32_t at = atomicAdd(&sh.n_keys, 1u);
                         if (at < kKeys) sh.keys[at] = ((uint64_t)k << 32) | (0xffffffffu - (i + q));
                     }
+                }
+            }
+            if (tid == 0 && skew_of(l)) { /* the row's extra logit */
+                const uint32_t k = rank_value(action_logit<T>(p, l, mask, 0));
+                if (k >= least) {
+                    const uint32_t at = atomicAdd(&sh.n_keys, 1u);
+                    if (at < kKeys) sh.keys[at] = ((uint64_t)k << 32) | 0xffffffffu;
                 }
             }
         }
@@ -608,7 +639,9 @@ __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks
     const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
     const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
     const uint32_t n = (uint32_t)p.n;
-    const uint32_t chunk_len = (uint32_t)chunk_vecs * kBlock * kPer, from = chunk * chunk_len + threadIdx.x * kPer;
+    const uint32_t skew = skew_of(l), chunk_len = (uint32_t)chunk_vecs * kBlock * kPer;
+    const uint32_t from = skew + chunk * chunk_len + threadIdx.x * kPer;
+    const float extra = skew && from == skew ? action_logit<T>(p, l, mask, 0) : -kInf;
     const int64_t a = kSplit ? -1 : row_action(p, r); /* asked for early: nothing waits for it behind the sums */
     const float la = kSplit ? 0.0f : action_logit<T>(p, l, mask, a);
     Running sum = running_start();
@@ -631,11 +664,12 @@ __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks
         w4 z = load_vec<T>(l, mask, from + (uint32_t)j * kStride, n);
         take_vecs<T, 1>(p, &z, sum);
     }
+    if (skew && from == skew) take_one(p, extra, sum);
     const float strip = lanes_max<kStripLanes>(sum.big);
     Sum v = team_merge<kBlock>(p, running_end(p, sum), lds);
     if (is_huge(p, v.big) && fabsf(v.big) < kInf) {
         __syncthreads();
-        v = team_merge<kBlock>(p, sum_slowly<T>(p, l, mask, from, kBlock * kPer, (chunk + 1) * chunk_len, n, v.big), lds);
+        v = team_merge<kBlock>(p, sum_slowly<T>(p, l, mask, from, kBlock * kPer, skew + (chunk + 1) * chunk_len, n, v.big, extra), lds);
     }
     if constexpr (kSplit) {
         if (p.top > 0 && threadIdx.x % kStripLanes == 0)
@@ -688,9 +722,6 @@ __global__ void __launch_bounds__(kBlock) k_policy_join(const Row p, int chunks,
         select_top<T>(p, r, l, mask, v, o, held, [&](int i) { return mine[i]; }, n_strips, chunk_vecs,
                       (uint32_t)chunk_vecs * kBlock * Kind<T>::kPer, top);
 }
-
-/* v_mul_legacy_f32: a product in which 0 times anything is 0 */
-__device__ float mul_zero_wins(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
 
 /* Gradient of one vector of a plain row, without the action's own part.  The product is the one in which 0 times anything is 0: an
  * exponential of 0 comes with an exponent of -inf where the logit is -inf. */
@@ -746,10 +777,10 @@ __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks
     const float la = action_logit<T>(p, l, mask, a);
     const Sum v{p.row_stats[2 * r], p.row_stats[2 * r + 1], 0.0f};
     const Slope q = row_slope(p, r, a, v, p.entropy[r], log2f(v.s));
-    const uint32_t n = (uint32_t)p.n, action = a >= 0 && a < p.n ? (uint32_t)a : ~0u, whole = n - n % kPer;
-    const uint32_t first = (uint32_t)chunk * chunk_vecs * kBlock * kPer, end = min(first + (uint32_t)chunk_vecs * kBlock * kPer, n);
+    const uint32_t n = (uint32_t)p.n, action = a >= 0 && a < p.n ? (uint32_t)a : ~0u, skew = skew_of(l), whole = n - (n - skew) % kPer;
+    const uint32_t first = skew + (uint32_t)chunk * chunk_vecs * kBlock * kPer, end = first + (uint32_t)chunk_vecs * kBlock * kPer;
     if (!is_plain(p, q)) {
-        slope_slowly<T, kBlock>(p, q, l, mask, out, first, end, action);
+        slope_slowly<T, kBlock>(p, q, l, mask, out, chunk ? first : 0, min(end, n), action);
         return;
     }
     const uint32_t from = first + threadIdx.x * kPer;
@@ -768,7 +799,8 @@ __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks
         const w4 x = load_vec<T>(l, mask, i, n);
         if (i < whole) store_vec<T>(out, i, slope_vec<T>(p, q, x));
     }
-    if (end == n) slope_slowly<T, kBlock>(p, q, l, mask, out, whole, n, action);
+    if (whole >= first && whole < end) slope_slowly<T, kBlock>(p, q, l, mask, out, whole, n, action);
+    if (chunk == 0) slope_slowly<T, kBlock>(p, q, l, mask, out, 0, skew, action);
     if (action >= first && action < min(end, whole) && (action - first) / kPer % kBlock == threadIdx.x) store_action<T>(p, q, la, out, action);
 }
 
@@ -788,14 +820,15 @@ __global__ void __launch_bounds__(kTeam <= 64 ? kBlock : kTeam, kTeam <= 64 ? 1 
                       : kTeam == 64 ? (int64_t)blockIdx.x * (kBlock / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
                                     : blockIdx.x;
     if (r >= p.rows) return; /* a whole team, and nothing below reaches past a team */
-    const uint32_t n = (uint32_t)p.n, lane = threadIdx.x % kTeam;
-    uint32_t from = lane * kPer;
     const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
     const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
+    const uint32_t n = (uint32_t)p.n, lane = threadIdx.x % kTeam, skew = kTeam > 64 ? skew_of(l) : 0u;
+    uint32_t from = skew + lane * kPer;
     w4 x[V];
     load_raw<T, V>(l, from, kStride, n, x);
     const int64_t a = row_action(p, r);
     const float la = action_logit<T>(p, l, mask, a); /* before the gradient may overwrite it */
+    const float extra = skew && lane == 0 ? action_logit<T>(p, l, mask, 0) : -kInf;
     Running sum = running_start();
     _Pragma("unroll") for (int j = 0; j < kGroups; ++j) {
         dress<T, kAhead>(mask, from + j * kAhead * kStride, kStride, n, x + j * kAhead);
@@ -805,17 +838,18 @@ __global__ void __launch_bounds__(kTeam <= 64 ? kBlock : kTeam, kTeam <= 64 ? 1 
         dress<T, kRest>(mask, from + kGroups * kAhead * kStride, kStride, n, x + kGroups * kAhead);
         take_vecs<T, kRest>(p, x + kGroups * kAhead, sum);
     }
+    if (skew && lane == 0) take_one(p, extra, sum);
     Sum v = team_merge<kTeam>(p, running_end(p, sum), lds);
     if (is_huge(p, v.big) && fabsf(v.big) < kInf) {
         if (kTeam > 64) __syncthreads();
-        v = team_merge<kTeam>(p, sum_slowly<T>(p, l, mask, from, kStride, n, n, v.big), lds);
+        v = team_merge<kTeam>(p, sum_slowly<T>(p, l, mask, from, kStride, n, n, v.big, extra), lds);
     }
     const Values o = row_values(p, v);
-    if (lane == 0) write_row(p, r, v, o, la, a);
+    if (lane == 0 && p.values) write_row(p, r, v, o, la, a);
     if constexpr (kGrad) {
         const Slope q = row_slope(p, r, a, v, o.entropy, o.log2_s);
         T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
-        const uint32_t action = a >= 0 && a < p.n ? (uint32_t)a : ~0u, whole = n - n % kPer;
+        const uint32_t action = a >= 0 && a < p.n ? (uint32_t)a : ~0u, whole = n - (n - skew) % kPer;
         if (!is_plain(p, q)) {
             slope_slowly<T, kTeam>(p, q, l, mask, out, 0, n, action);
             return;
@@ -829,7 +863,9 @@ __global__ void __launch_bounds__(kTeam <= 64 ? kBlock : kTeam, kTeam <= 64 ? 1 
         }
         const uint32_t end = kTeam < 64 ? n : whole;
         if (kTeam >= 64) slope_slowly<T, kTeam>(p, q, l, mask, out, whole, n, action);
-        if (action < end && action / kPer % kTeam == lane) store_action<T>(p, q, la, out, action);
+        if (skew && lane == 0)
+            Kind<T>::store(out, extra == -kInf ? 0.0f : slope_at(p, q, extra) + (action == 0 ? q.at_action : 0.0f));
+        if (action >= skew && action < end && (action - skew) / kPer % kTeam == lane) store_action<T>(p, q, la, out, action);
     }
 }
 
@@ -864,12 +900,14 @@ Row pack(const mzs_policy_args& a) {
     p.rows = a.rows, p.n = a.n_actions;
     p.logits_stride = a.logits_stride, p.mask_stride = a.mask_stride, p.grad_stride = a.grad_stride;
     p.action_bytes = a.action_bytes, p.top = a.top;
-    p.scale = a.inverse_temperature;
+    p.scale = a.inverse_temperature, p.values = 1;
     p.c = (float)((double)a.inverse_temperature * kLog2e);
     return p;
 }
 
 constexpr int64_t kLanesMost = 1024; /* widest row of k_policy_lanes */
+/* widest row whose gradient sums the row again in registers rather than read its statistics back */
+constexpr int64_t kRegainMost = 2048;
 
 /* how a wide row is cut: `chunks` blocks a row, each thread `vecs` vectors */
 struct Cut {
@@ -884,7 +922,7 @@ Cut cut_row(int64_t rows, int64_t n, int per, bool join) {
     if (chunks > all) chunks = all;
     Cut c;
     c.vecs = (int)((all + chunks - 1) / chunks);
-    if (c.vecs > kAhead) c.vecs = (c.vecs + kAhead - 1) / kAhead * kAhead; /* whole groups */
+    if (chunks > 1 && c.vecs > kAhead) c.vecs = (c.vecs + kAhead - 1) / kAhead * kAhead; /* whole groups */
     c.chunks = (int)((all + c.vecs - 1) / c.vecs);
     return c;
 }
@@ -897,7 +935,7 @@ void launch_lanes(const Row& p, hipStream_t st) {
     };
     if (p.n <= 4) go(k_policy_lanes<T, 1, 4, kForward, kGrad, kTop>, 256);
     else if (p.n <= 8) go(k_policy_lanes<T, 1, 8, kForward, kGrad, kTop>, 256);
-    else if constexpr (kTop || !kForward) {
+    else if constexpr (kTop) {
         if (p.n <= 16) go(k_policy_lanes<T, 4, 4, kForward, kGrad, kTop>, 64);
         else if (p.n <= 64) go(k_policy_lanes<T, 16, 4, kForward, kGrad, kTop>, 16);
         else if (p.n <= 256) go(k_policy_lanes<T, 16, 16, kForward, kGrad, kTop>, 16);
@@ -989,7 +1027,7 @@ Row rows_from(Row p, int64_t r, int64_t rows) {
 /* The ways, by the width of the row (and how a call needs it):
  *   up to 8 logits              a lane a row, a logit at a time                             k_policy_lanes
  *   up to 16 vectors a lane     a row in a team's registers, without alternatives           k_policy_row, teams up to a wave
- *   up to 1024                  alternatives, or the gradient from stored statistics        k_policy_lanes
+ *   up to 1024                  alternatives                                                k_policy_lanes
  *   up to 24 vectors a thread   forward and gradient of a row in a block's registers        k_policy_row, a block
  *   beyond                      chunks and their join; the gradient from the statistics     k_policy_chunk, k_policy_join, k_policy_slope */
 template <typename T>
@@ -1018,7 +1056,10 @@ void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool for
             else launch_forward<T>(p, a, st);
         }
         if (grad) {
-            if (lanes) launch_lanes<T, false, true, false>(p, st);
+            Row g = p;
+            g.values = 0;
+            if (wave && p.n <= kRegainMost) launch_wave_row<T, true>(g, st);
+            else if (p.n <= 8) launch_lanes<T, false, true, false>(p, st);
             else launch_slope<T>(p, st);
         }
     }
