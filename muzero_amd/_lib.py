@@ -6,6 +6,8 @@ fails, this module raises.
 import ctypes as C
 import os
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # MZS_LIB selects an alternative build of the same library (kernel A/B experiments)
 LIB_PATH = os.environ.get("MZS_LIB") or os.path.join(_HERE, "libmzsearch.so")
@@ -48,7 +50,7 @@ class Config(C.Structure):
 
 
 DTYPE_FLOAT, DTYPE_BFLOAT, DTYPE_HALF = 0, 1, 2
-POLICY_MAX_TOP = 32
+POLICY_MAX_TOP, POLICY_NARROW, POLICY_MANY = 32, 1024, 256
 OPTIM_ALIGN, OPTIM_BLOCK, OPTIM_ENTRY_BYTES, OPTIM_CONTROL_BYTES = 64, 32, 32, 64
 
 
@@ -174,6 +176,11 @@ def load():
             fn.restype, fn.argtypes = res, args
         _lib = lib
     return _lib
+
+
+def raw_stream(device_index):
+    """hipStream_t (an integer) of torch's current stream on a device."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def check(rc, what):

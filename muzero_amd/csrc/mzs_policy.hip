@@ -764,40 +764,39 @@ __device__ __forceinline__ void store_action(const Row& p, const Slope& q, float
     if (la != -kInf) Kind<T>::store(out + action, slope_at(p, q, la) + q.at_action);
 }
 
-/* gradient of chunks from the rows' stored statistics */
-template <typename T>
-__global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks, int chunk_vecs) {
+/* Gradient of chunks from the rows' stored statistics; kSlopeGroups groups of vectors a thread, each on its way while the one before it is
+ * worked on, the first while the row's statistics come.  1280 x 59049 fp16: 48.8 us with four groups, 52.8 with two, 54.6 with
+ * one, which few rows get for the sake of more blocks. */
+template <typename T, int kSlopeGroups>
+__global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks) {
     constexpr int kPer = Kind<T>::kPer;
+    constexpr uint32_t kStride = kBlock * kPer, kLen = kSlopeGroups * kAhead * kStride;
     const int64_t r = blockIdx.x / chunks;
     const int chunk = blockIdx.x % chunks;
     const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
     const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
     T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
+    const uint32_t n = (uint32_t)p.n, skew = skew_of(l), whole = n - (n - skew) % kPer;
+    const uint32_t first = skew + (uint32_t)chunk * kLen, end = first + kLen, from = first + threadIdx.x * kPer;
+    w4 x[2][kAhead];
+    load_raw<T, kAhead>(l, from, kStride, n, x[0]);
     const int64_t a = row_action(p, r);
     const float la = action_logit<T>(p, l, mask, a);
     const Sum v{p.row_stats[2 * r], p.row_stats[2 * r + 1], 0.0f};
     const Slope q = row_slope(p, r, a, v, p.entropy[r], log2f(v.s));
-    const uint32_t n = (uint32_t)p.n, action = a >= 0 && a < p.n ? (uint32_t)a : ~0u, skew = skew_of(l), whole = n - (n - skew) % kPer;
-    const uint32_t first = skew + (uint32_t)chunk * chunk_vecs * kBlock * kPer, end = first + (uint32_t)chunk_vecs * kBlock * kPer;
+    const uint32_t action = a >= 0 && a < p.n ? (uint32_t)a : ~0u;
     if (!is_plain(p, q)) {
         slope_slowly<T, kBlock>(p, q, l, mask, out, chunk ? first : 0, min(end, n), action);
         return;
     }
-    const uint32_t from = first + threadIdx.x * kPer;
-    int j = 0;
-    for (; j + kAhead <= chunk_vecs; j += kAhead) {
-        w4 x[kAhead];
-        const uint32_t i = from + (uint32_t)j * kBlock * kPer;
-        load_vecs<T, kAhead>(l, mask, i, kBlock * kPer, n, x);
+    _Pragma("unroll") for (int g = 0; g < kSlopeGroups; ++g) {
+        const uint32_t i = from + g * kAhead * kStride;
+        if (g + 1 < kSlopeGroups) load_raw<T, kAhead>(l, i + kAhead * kStride, kStride, n, x[(g + 1) & 1]);
+        dress<T, kAhead>(mask, i, kStride, n, x[g & 1]);
         _Pragma("unroll") for (int u = 0; u < kAhead; ++u) {
-            const uint32_t at = i + u * kBlock * kPer;
-            if (at < whole) store_vec<T>(out, at, slope_vec<T>(p, q, x[u]));
+            const uint32_t at = i + u * kStride;
+            if (at < whole) store_vec<T>(out, at, slope_vec<T>(p, q, x[g & 1][u]));
         }
-    }
-    for (; j < chunk_vecs; ++j) {
-        const uint32_t i = from + (uint32_t)j * kBlock * kPer;
-        const w4 x = load_vec<T>(l, mask, i, n);
-        if (i < whole) store_vec<T>(out, i, slope_vec<T>(p, q, x));
     }
     if (whole >= first && whole < end) slope_slowly<T, kBlock>(p, q, l, mask, out, whole, n, action);
     if (chunk == 0) slope_slowly<T, kBlock>(p, q, l, mask, out, 0, skew, action);
@@ -905,20 +904,21 @@ Row pack(const mzs_policy_args& a) {
     return p;
 }
 
-constexpr int64_t kLanesMost = 1024; /* widest row of k_policy_lanes */
+constexpr int64_t kLanesMost = MZS_POLICY_NARROW; /* widest row of k_policy_lanes */
 /* widest row whose gradient sums the row again in registers rather than read its statistics back */
 constexpr int64_t kRegainMost = 2048;
 
-/* how a wide row is cut: `chunks` blocks a row, each thread `vecs` vectors */
+/* How a wide row is cut: `chunks` blocks a row, each thread `vecs` vectors.  Rows are cut where there are fewer of them than CUs: from
+ * there on a block a row keeps up (us without / with the five best alternatives, 320 x 59049 bf16: 15 / 21 whole, 20 / 25 cut; 1280 x
+ * 20000: 16 / 21 and 20 / 27; 640 x 100000 the same; 160 x 100000 fp32: 19 / 24 cut). */
 struct Cut {
     int chunks, vecs;
 };
-Cut cut_row(int64_t rows, int64_t n, int per, bool join) {
+Cut cut_row(int64_t rows, int64_t n, int per) {
     const int64_t all = (n + (int64_t)kBlock * per - 1) / ((int64_t)kBlock * per); /* vectors a thread would have of a whole row */
     int64_t chunks = 1;
-    if (!join) chunks = (all + kAhead - 1) / kAhead;                                /* independent: four vectors a thread each */
-    else if (rows < 2048) chunks = (8192 + rows - 1) / rows;
-    if (join && chunks > kBlock) chunks = kBlock;
+    if (rows < MZS_POLICY_MANY) chunks = (8192 + rows - 1) / rows;
+    if (chunks > kBlock) chunks = kBlock;
     if (chunks > all) chunks = all;
     Cut c;
     c.vecs = (int)((all + chunks - 1) / chunks);
@@ -945,7 +945,7 @@ void launch_lanes(const Row& p, hipStream_t st) {
 
 template <typename T>
 void launch_forward(const Row& p, const mzs_policy_args& a, hipStream_t st) {
-    const Cut c = cut_row(p.rows, p.n, Kind<T>::kPer, true);
+    const Cut c = cut_row(p.rows, p.n, Kind<T>::kPer);
     if (c.chunks == 1) {
         hipLaunchKernelGGL((k_policy_chunk<T, false>), dim3((unsigned)p.rows), dim3(kBlock), 0, st, p, 1, c.vecs, nullptr, nullptr);
         return;
@@ -958,8 +958,13 @@ void launch_forward(const Row& p, const mzs_policy_args& a, hipStream_t st) {
 }
 template <typename T>
 void launch_slope(const Row& p, hipStream_t st) {
-    const Cut c = cut_row(p.rows, p.n, Kind<T>::kPer, false);
-    hipLaunchKernelGGL(k_policy_slope<T>, dim3((unsigned)(p.rows * c.chunks)), dim3(kBlock), 0, st, p, c.chunks, c.vecs);
+    const int64_t group = (int64_t)kAhead * kBlock * Kind<T>::kPer, groups = (p.n + group - 1) / group;
+    if (p.rows * groups < 4096) {
+        hipLaunchKernelGGL((k_policy_slope<T, 1>), dim3((unsigned)(p.rows * groups)), dim3(kBlock), 0, st, p, (int)groups);
+    } else {
+        const int chunks = (int)((groups + 3) / 4);
+        hipLaunchKernelGGL((k_policy_slope<T, 4>), dim3((unsigned)(p.rows * chunks)), dim3(kBlock), 0, st, p, chunks);
+    }
 }
 
 /* rows in registers: up to kWaveVecs vectors a lane of a wave, kRowVecs a thread of a block of kRowThreads */
@@ -1066,8 +1071,8 @@ void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool for
 }
 
 size_t workspace_bytes(const mzs_policy_args& a, int per) {
-    if (a.rows == 0 || a.n_actions <= kLanesMost) return 0;
-    const Cut c = cut_row(a.rows, a.n_actions, per, true);
+    if (a.rows == 0 || a.n_actions <= kLanesMost) return 0; /* MZS_POLICY_NARROW */
+    const Cut c = cut_row(a.rows, a.n_actions, per);
     if (c.chunks == 1) return 0;
     return sizeof(float) * (size_t)a.rows * c.chunks * (3 + (a.top > 0 ? kStripsPerBlock : 0));
 }

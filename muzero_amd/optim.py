@@ -13,10 +13,6 @@ from . import _lib
 _DTYPES = {torch.float32: _lib.DTYPE_FLOAT, torch.bfloat16: _lib.DTYPE_BFLOAT, torch.float16: _lib.DTYPE_HALF}
 
 
-def _stream(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
 def _check_tensors(tensors, what):
     if not tensors:
         raise ValueError(f"{what}: an empty list")
@@ -43,7 +39,8 @@ class _Table:
         self.memory = torch.empty((n + 1) * _lib.OPTIM_ENTRY_BYTES, dtype=torch.uint8, device=device)
         tiles = C.c_int64()
         _lib.check(_lib.load().mzs_optim_table(device.index, n, (C.c_void_p * n)(*pointers), (C.c_int64 * n)(*counts),
-                                               self.memory.data_ptr(), C.byref(tiles), _stream(device)), "mzs_optim_table")
+                                               self.memory.data_ptr(), C.byref(tiles), _lib.raw_stream(device.index)),
+                   "mzs_optim_table")
         self.n, self.tiles, self.ptr = n, tiles.value, self.memory.data_ptr()
 
 
@@ -62,40 +59,40 @@ class TensorList:
         self.counts = tuple(t.numel() for t in tensors)
         self.table = _Table(self.device, [t.data_ptr() for t in tensors], self.counts)
         # the table is written on this stream: a user on another one waits for it
-        self._stream = torch.cuda.current_stream(self.device)
+        stream = torch.cuda.current_stream(self.device)
         self._ready = torch.cuda.Event()
-        self._ready.record(self._stream)
-        self._waited = {self._stream}
+        self._ready.record(stream)
+        self._waited = {stream.cuda_stream}
 
     def __len__(self):
         return len(self.counts)
 
-    def _wait(self, stream):
-        if stream not in self._waited:
+    def _wait(self, raw_stream):
+        if raw_stream not in self._waited:
             self._ready.synchronize()       # once per stream; on the host, so that a capture records nothing of it
-            self.table.memory.record_stream(stream)
-            self._waited.add(stream)
+            self.table.memory.record_stream(torch.cuda.current_stream(self.device))
+            self._waited.add(raw_stream)
 
 
-@torch.no_grad()
 def grad_norm(grads, scale=1.0):
     """sqrt of the sum of squares over all gradients, times |scale|: a 0-d float32 tensor, summed in fp64 in a fixed order.
     grads: a tensor, a list of tensors of one type (None: left out), or a TensorList."""
     if isinstance(grads, TensorList):
         dev, dtype, table = grads.device, grads.dtype, grads.table
-        stream = torch.cuda.current_stream(dev)
-        grads._wait(stream)
+        stream = _lib.raw_stream(dev.index)
+        if stream not in grads._waited:
+            grads._wait(stream)
     else:
         grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
         _check_tensors(grads, "grads")
         dev, dtype = grads[0].device, grads[0].dtype
         table = _Table(dev, [g.data_ptr() for g in grads], [g.numel() for g in grads])
-        stream = torch.cuda.current_stream(dev)
+        stream = _lib.raw_stream(dev.index)
     lib = _lib.load()
     size = lib.mzs_grad_norm_workspace(table.tiles)
     memory = torch.empty(size // 4 + 1, dtype=torch.float32, device=dev)
     _lib.check(lib.mzs_grad_norm(dev.index, table.n, table.ptr, table.tiles, _DTYPES[dtype], float(scale),
-                                 memory.data_ptr() + size, memory.data_ptr(), size, stream.cuda_stream), "mzs_grad_norm")
+                                 memory.data_ptr() + size, memory.data_ptr(), size, stream), "mzs_grad_norm")
     return memory[size // 4]
 
 
@@ -228,13 +225,12 @@ class AdamW:
                 raise ValueError(f"grads[{i}]: {g.numel()} elements, the parameter has {c}")
         return _Table(self.device, [None if g is None else g.data_ptr() for g in grads], self.counts), there[0].dtype
 
-    @torch.no_grad()
     def step(self, grads=None, norm=None, grad_scale=1.0):
         """One step on the current stream.  grads: a list (None entries: no gradient), a TensorList, or None: the parameters'
         .grad.  norm: the norm to clip by (a 0-d float32 tensor) where it covers more than these parameters; None: computed
         here when max_grad_norm is set.  grad_scale multiplies the gradients (1 / loss scale).  grad_norm holds the norm."""
-        stream = torch.cuda.current_stream(self.device)
-        if isinstance(grads, TensorList):
+        stream = _lib.raw_stream(self.device.index)
+        if isinstance(grads, TensorList) and stream not in grads._waited:
             grads._wait(stream)
         table, dtype = self._grad_table(grads)
         pointers = [p.data_ptr() for p in self.params]
@@ -265,5 +261,5 @@ class AdamW:
                 raise ValueError("norm: one float32 value on the parameters' device")
             self.grad_norm.copy_(norm.reshape(()))
             a.norm_given = 1
-        _lib.check(_lib.load().mzs_adamw_step(C.byref(a), stream.cuda_stream), "mzs_adamw_step")
+        _lib.check(_lib.load().mzs_adamw_step(C.byref(a), stream), "mzs_adamw_step")
         torch.autograd.graph.increment_version(self.params)

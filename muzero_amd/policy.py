@@ -9,6 +9,7 @@ for the few actions of one environment; the actions of a Box space are the carte
 There is no CPU path: tensors that are not on a GPU are refused.
 """
 import ctypes as C
+import struct
 from typing import NamedTuple
 
 import torch
@@ -27,6 +28,21 @@ class PolicyLogProbs(NamedTuple):
     top_action: torch.Tensor    # int32; equal logits: the lower index first; -1 behind the last allowed action
 
 
+# mzs_policy_args as one packed block: filling it field by field through ctypes costs more than the launch
+_ARGS = struct.Struct("@iiqqPqPqPiifxxxxPPPPPPPPPPqPN")
+assert _ARGS.size == C.sizeof(_lib.PolicyArgs)
+_calls = {}
+
+
+def _call(name):
+    f = _calls.get(name)
+    if f is None:
+        f = _lib.load()[name]       # a function object of its own: the binding in _lib takes the structure
+        f.restype, f.argtypes = C.c_int, [C.c_char_p, C.c_void_p]
+        _calls[name] = f
+    return f
+
+
 def _check(logits, actions, mask, temperature, top):
     if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
         raise ValueError("logits: a tensor [..., n_actions]")
@@ -34,24 +50,24 @@ def _check(logits, actions, mask, temperature, top):
         raise _lib.MzsError("policy_log_probs: logits must be on a GPU (there is no CPU path)")
     if logits.dtype not in _DTYPES:
         raise ValueError(f"logits are {logits.dtype}: float32, bfloat16 or float16")
-    n = logits.shape[-1]
+    shape = logits.shape
+    n = shape[-1]
     if not 1 <= n <= 2 ** 28:
         raise ValueError(f"{n} actions: 1 .. 2^28")
     if not 1e-30 <= temperature < float("inf"):
         raise ValueError(f"temperature={temperature!r}: positive and finite (at least 1e-30)")
     if not 0 <= top <= _lib.POLICY_MAX_TOP:
         raise ValueError(f"top={top!r}: 0 .. {_lib.POLICY_MAX_TOP}")
-    lead = logits.shape[:-1]
     if actions is not None:
         if actions.dtype not in (torch.int64, torch.int32):
             raise ValueError(f"actions are {actions.dtype}: int64 or int32")
-        if actions.shape != lead or actions.device != logits.device:
-            raise ValueError(f"actions {tuple(actions.shape)} on {actions.device}: expected {tuple(lead)} on {logits.device}")
+        if actions.shape != shape[:-1] or actions.device != logits.device:
+            raise ValueError(f"actions {tuple(actions.shape)} on {actions.device}: expected {tuple(shape[:-1])} on {logits.device}")
     if mask is not None:
         if mask.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"mask is {mask.dtype}: bool (or uint8, 0 / 1)")
-        if mask.device != logits.device or mask.shape not in (logits.shape, logits.shape[-1:]):
-            raise ValueError(f"mask {tuple(mask.shape)} on {mask.device}: expected {tuple(logits.shape)} or ({n},) on {logits.device}")
+        if mask.device != logits.device or mask.shape not in (shape, shape[-1:]):
+            raise ValueError(f"mask {tuple(mask.shape)} on {mask.device}: expected {tuple(shape)} or ({n},) on {logits.device}")
 
 
 def _rows(t, n):
@@ -59,9 +75,11 @@ def _rows(t, n):
     has no such form."""
     if t.dim() != 2:
         t = t.reshape(-1, n)
-    if (n > 1 and t.stride(1) != 1) or t.stride(0) < 0:
+    pitch, step = t.stride()
+    if (n > 1 and step != 1) or pitch < 0:
         t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else n)
+        pitch = n
+    return t, (pitch if t.shape[0] > 1 else n)
 
 
 def _coefficient(g, name, lead, device):
@@ -69,94 +87,91 @@ def _coefficient(g, name, lead, device):
         return None
     if g.shape != lead or g.device != device:
         raise ValueError(f"{name} {tuple(g.shape)} on {g.device}: expected {tuple(lead)} on {device}")
-    return g.to(torch.float32).contiguous()
+    return g if g.dtype is torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()
 
 
-class _Call:
-    """The tensors of one library call and its argument block."""
-
-    def __init__(self, logits, actions, mask, temperature, top):
-        self.lead, self.device = logits.shape[:-1], logits.device
-        n = logits.shape[-1]
-        self.logits, stride = _rows(logits, n)
-        self.rows = self.logits.shape[0]
-        a = self.args = _lib.PolicyArgs()
-        a.device, a.dtype, a.rows, a.n_actions = self.device.index, _DTYPES[logits.dtype], self.rows, n
-        a.logits, a.logits_stride = self.logits.data_ptr(), stride
-        a.inverse_temperature, a.top = 1.0 / temperature, top
-        self.actions = self.mask = None
-        if actions is not None:
-            self.actions = actions.contiguous()
-            a.action, a.action_bytes = self.actions.data_ptr(), self.actions.element_size()
-        if mask is not None:
-            if mask.dim() == 1 and len(self.lead) != 0:
-                self.mask, a.mask_stride = mask.contiguous(), 0
-            else:
-                self.mask, a.mask_stride = _rows(mask, n)
-            a.mask = self.mask.data_ptr()
-
-    def outputs(self):
-        a, top = self.args, self.args.top
-        flat = torch.empty(5 * self.rows, dtype=torch.float32, device=self.device)
-        at = flat.data_ptr()
-        a.log_prob, a.entropy, a.log_z, a.row_stats = at, at + 4 * self.rows, at + 8 * self.rows, at + 12 * self.rows
-        lp, h, z, self.stats = flat.split((self.rows, self.rows, self.rows, 2 * self.rows))
-        self.entropy = h
-        tl = ta = None
+def _run(name, logits, actions, mask, temperature, top, saved=None, upstream=None, out=None, apart=False):
+    """One library call.  saved: (entropy, row statistics) of an earlier forward pass, or None: forward values are made here.  upstream:
+    the gradient's coefficients, or None: no gradient.  Returns (PolicyLogProbs or None, row statistics, gradient or None)."""
+    shape, device = logits.shape, logits.device
+    n, dim = shape[-1], logits.dim()
+    rows_of, pitch = _rows(logits, n)
+    rows = rows_of.shape[0]
+    mask_ptr = mask_pitch = action_ptr = action_bytes = 0
+    if actions is not None:
+        if not actions.is_contiguous():
+            actions = actions.contiguous()
+        action_ptr, action_bytes = actions.data_ptr(), actions.element_size()
+    if mask is not None:
+        if mask.dim() == 1 and dim != 1:
+            mask = mask.contiguous()
+        else:
+            mask, mask_pitch = _rows(mask, n)
+        mask_ptr = mask.data_ptr()
+    values = stats = None
+    top_lp = top_at = grad = None
+    lp = h = z = st = tl = ta = 0
+    if saved is None:
+        if apart:       # autograd's outputs are no views of one tensor
+            log_prob, entropy, log_z, stats = (torch.empty(s, dtype=torch.float32, device=device)
+                                               for s in (shape[:-1], shape[:-1], shape[:-1], (rows, 2)))
+            lp, h, z, st = log_prob.data_ptr(), entropy.data_ptr(), log_z.data_ptr(), stats.data_ptr()
+        else:
+            flat = torch.empty((5, rows), dtype=torch.float32, device=device)
+            log_prob, entropy, log_z, _, _ = flat.unbind()
+            lp = flat.data_ptr()
+            h, z, st = lp + 4 * rows, lp + 8 * rows, lp + 12 * rows
+            if dim != 2:
+                lead = shape[:-1]
+                log_prob, entropy, log_z = log_prob.view(lead), entropy.view(lead), log_z.view(lead)
         if top:
-            tl = torch.empty(self.lead + (top,), dtype=torch.float32, device=self.device)
-            ta = torch.empty(self.lead + (top,), dtype=torch.int32, device=self.device)
-            a.top_log_prob, a.top_action = tl.data_ptr(), ta.data_ptr()
-        if len(self.lead) != 1:
-            lp, h, z = (t.view(self.lead) for t in (lp, h, z))
-        return PolicyLogProbs(lp, h, z, tl, ta)
-
-    def gradient(self, grad_log_prob, grad_entropy, grad_log_z, out=None):
-        a = self.args
-        self.upstream = (grad_log_prob, grad_entropy, grad_log_z)
-        a.grad_log_prob, a.grad_entropy, a.grad_log_z = (None if g is None else g.data_ptr() for g in self.upstream)
-        if out is None:
-            out = torch.empty(self.lead + (a.n_actions,), dtype=self.logits.dtype, device=self.device)
-        rows = out if out.dim() == 2 else out.view(-1, a.n_actions)
-        a.grad_logits, a.grad_stride = out.data_ptr(), rows.stride(0)
-        return out
-
-    def run(self, name):
-        lib = _lib.load()
-        if self.rows == 0:
-            return
-        size = C.c_size_t()
-        _lib.check(lib.mzs_policy_workspace(C.byref(self.args), C.byref(size)), "mzs_policy_workspace")
-        if size.value:
-            self.workspace = torch.empty(size.value, dtype=torch.uint8, device=self.device)
-            self.args.workspace, self.args.workspace_bytes = self.workspace.data_ptr(), size.value
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        _lib.check(getattr(lib, name)(C.byref(self.args), C.c_void_p(stream)), name)
+            top_lp = torch.empty(shape[:-1] + (top,), dtype=torch.float32, device=device)
+            top_at = torch.empty(shape[:-1] + (top,), dtype=torch.int32, device=device)
+            tl, ta = top_lp.data_ptr(), top_at.data_ptr()
+        values = PolicyLogProbs(log_prob, entropy, log_z, top_lp, top_at)
+    else:
+        h, st = saved[0].data_ptr(), saved[1].data_ptr()
+    g_lp = g_h = g_z = g = g_pitch = 0
+    if upstream is not None:
+        g_lp, g_h, g_z = (0 if u is None else u.data_ptr() for u in upstream)
+        grad = torch.empty(shape, dtype=logits.dtype, device=device) if out is None else out
+        g, g_pitch = grad.data_ptr(), (grad.stride(0) if dim == 2 else n)
+    if rows:
+        args = [device.index, _DTYPES[logits.dtype], rows, n, rows_of.data_ptr(), pitch, mask_ptr, mask_pitch, action_ptr, action_bytes,
+                top, 1.0 / temperature, lp, h, z, st, tl, ta, g_lp, g_h, g_z, g, g_pitch, 0, 0]
+        if n > _lib.POLICY_NARROW and rows < _lib.POLICY_MANY and saved is None:
+            size = C.c_size_t()
+            _lib.check(_lib.load().mzs_policy_workspace(_lib.PolicyArgs.from_buffer_copy(_ARGS.pack(*args)), C.byref(size)),
+                       "mzs_policy_workspace")
+            if size.value:
+                workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
+                args[-2:] = workspace.data_ptr(), size.value
+        rc = _call(name)(_ARGS.pack(*args), _lib.raw_stream(device.index))
+        if rc:
+            _lib.check(rc, name)
+    return values, stats, grad
 
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, mask, temperature, top):
-        call = _Call(logits, actions, mask, temperature, top)
-        out = call.outputs()
-        call.run("mzs_policy_log_probs")
-        ctx.save_for_backward(logits, actions, mask, out.entropy, call.stats)
+        out, stats, _ = _run("mzs_policy_log_probs", logits, actions, mask, temperature, top, apart=True)
+        ctx.save_for_backward(logits, actions, mask, out.entropy, stats)
         ctx.temperature = temperature
-        ctx.mark_non_differentiable(*(t for t in out[3:] if t is not None))
+        if top:
+            ctx.mark_non_differentiable(out.top_log_prob, out.top_action)
         ctx.set_materialize_grads(False)
         return tuple(out)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_log_prob, g_entropy, g_log_z, *_):
-        logits, actions, mask, entropy, stats = ctx.saved_tensors
-        call = _Call(logits, actions, mask, ctx.temperature, 0)
         if g_log_prob is None and g_entropy is None and g_log_z is None:
             return None, None, None, None, None
-        grads = (_coefficient(g, "gradient", call.lead, call.device) for g in (g_log_prob, g_entropy, g_log_z))
-        call.args.entropy, call.args.row_stats = entropy.data_ptr(), stats.data_ptr()
-        grad = call.gradient(*grads)
-        call.run("mzs_policy_log_probs_grad")
+        logits, actions, mask, entropy, stats = ctx.saved_tensors
+        lead, device = logits.shape[:-1], logits.device
+        upstream = [_coefficient(g, "gradient", lead, device) for g in (g_log_prob, g_entropy, g_log_z)]
+        _, _, grad = _run("mzs_policy_log_probs_grad", logits, actions, mask, ctx.temperature, 0, (entropy, stats), upstream)
         return grad, None, None, None, None
 
 
@@ -174,13 +189,9 @@ def policy_log_probs(logits, actions=None, mask=None, temperature=1.0, top=0):
             raise ValueError("policy_log_probs: a differentiable call is not captured into a graph (its backward pass would meet the "
                              "leaves' eager streams there, which ends the process); capture policy_log_probs_grad, or detach the logits")
         return PolicyLogProbs(*_LogProbs.apply(logits, actions, mask, float(temperature), int(top)))
-    call = _Call(logits, actions, mask, float(temperature), int(top))
-    out = call.outputs()
-    call.run("mzs_policy_log_probs")
-    return out
+    return _run("mzs_policy_log_probs", logits, actions, mask, float(temperature), int(top))[0]
 
 
-@torch.no_grad()
 def policy_log_probs_grad(logits, actions=None, grad_log_prob=None, grad_entropy=None, grad_log_z=None, mask=None,
                           temperature=1.0, top=0, out=None):
     """(PolicyLogProbs, gradient of sum(grad_log_prob * log_prob + grad_entropy * entropy + grad_log_z * log_z) by the logits) in
@@ -198,10 +209,8 @@ def policy_log_probs_grad(logits, actions=None, grad_log_prob=None, grad_entropy
             raise ValueError("out: rows must be dense and apart")
         if out.data_ptr() == logits.data_ptr() and out.stride() != logits.stride():
             raise ValueError("out: in place of the logits it must be the logits' own view")
-    call = _Call(logits, actions, mask, float(temperature), int(top))
-    values = call.outputs()
-    grad = call.gradient(*coefficients, out=out)
-    call.run("mzs_policy_log_probs_train")
+    values, _, grad = _run("mzs_policy_log_probs_train", logits, actions, mask, float(temperature), int(top), None,
+                           coefficients, out)
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return values, grad
