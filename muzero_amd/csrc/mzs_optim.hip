@@ -67,22 +67,36 @@ __device__ __forceinline__ uint32_t pack_halves(float a, float b, _Float16) {
 template <typename T>
 struct Quad { /* as it comes from memory */
     w2 raw;
-    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const w2*>(p); }
+    template <bool kStream>
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kStream) raw = __builtin_nontemporal_load(reinterpret_cast<const w2*>(p));
+        else raw = *reinterpret_cast<const w2*>(p);
+    }
     __device__ __forceinline__ float get(int j) const {
         const uint32_t v = j < 2 ? raw.x : raw.y;
         return j & 1 ? high_half(v, T()) : low_half(v, T());
     }
+    template <bool kStream>
     static __device__ __forceinline__ void store(T* p, const float* v) {
-        *reinterpret_cast<w2*>(p) = w2{pack_halves(v[0], v[1], T()), pack_halves(v[2], v[3], T())};
+        const w2 x{pack_halves(v[0], v[1], T()), pack_halves(v[2], v[3], T())};
+        if constexpr (kStream) __builtin_nontemporal_store(x, reinterpret_cast<w2*>(p));
+        else *reinterpret_cast<w2*>(p) = x;
     }
 };
 template <>
 struct Quad<float> {
     f4 raw;
-    __device__ __forceinline__ void load(const float* p) { raw = *reinterpret_cast<const f4*>(p); }
+    template <bool kStream>
+    __device__ __forceinline__ void load(const float* p) {
+        if constexpr (kStream) raw = __builtin_nontemporal_load(reinterpret_cast<const f4*>(p));
+        else raw = *reinterpret_cast<const f4*>(p);
+    }
     __device__ __forceinline__ float get(int j) const { return raw[j]; }
+    template <bool kStream>
     static __device__ __forceinline__ void store(float* p, const float* v) {
-        *reinterpret_cast<f4*>(p) = f4{v[0], v[1], v[2], v[3]};
+        const f4 x{v[0], v[1], v[2], v[3]};
+        if constexpr (kStream) __builtin_nontemporal_store(x, reinterpret_cast<f4*>(p));
+        else *reinterpret_cast<f4*>(p) = x;
     }
 };
 
@@ -104,20 +118,19 @@ __device__ __forceinline__ int find_tensor(const Entry* __restrict__ table, int 
 
 /* fixed-order sum over the block; the total in thread 0 */
 __device__ __forceinline__ double block_sum(double v, double* lds) {
-    lds[threadIdx.x] = v;
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    for (int w = kBlock / 2; w > 0; w >>= 1) {
-        if ((int)threadIdx.x < w) lds[threadIdx.x] += lds[threadIdx.x + w];
-        __syncthreads();
-    }
-    return lds[0];
+    double sum = 0.0;
+    for (int w = 0; w < kBlock / 64; ++w) sum += lds[w];
+    return sum;
 }
 
 /* squares of elements [from, to) of one tensor, this thread's share, in fp64 (fp32 squares overflow from 1.8e19 on and vanish
  * below 1e-23; the fp64 fma runs at the fp32 rate here, so the loads bound it either way) */
-template <typename G>
+template <typename G, bool kStream>
 __device__ __forceinline__ double sum_squares(const G* __restrict__ g, int64_t from, int64_t to, int thread, int threads) {
-    constexpr int kUnroll = 4;
+    constexpr int kUnroll = 2; /* 300M bf16: 107 us; 117 with four, 123 with eight: more waves do more than more loads each */
     constexpr int kWide = sizeof(G) == 4 ? 4 : 8; /* 16 bytes */
     double sum[2] = {0.0, 0.0};
     int64_t i = from + (int64_t)thread * kWide;
@@ -126,9 +139,12 @@ __device__ __forceinline__ double sum_squares(const G* __restrict__ g, int64_t f
         Quad<G> q[kUnroll][kWide / 4];
         _Pragma("unroll") for (int u = 0; u < kUnroll; ++u) {
             if constexpr (kWide == 4) {
-                q[u][0].load(g + i + u * step);
+                q[u][0].template load<kStream>(g + i + u * step);
             } else {
-                const w4 raw = *reinterpret_cast<const w4*>(g + i + u * step);
+                const w4* at = reinterpret_cast<const w4*>(g + i + u * step);
+                w4 raw;
+                if constexpr (kStream) raw = __builtin_nontemporal_load(at);
+                else raw = *at;
                 q[u][0].raw = w2{raw.x, raw.y}, q[u][1].raw = w2{raw.z, raw.w};
             }
         }
@@ -149,11 +165,13 @@ __device__ __forceinline__ double sum_squares(const G* __restrict__ g, int64_t f
 }
 
 /* One read of everything: a block takes a run of consecutive tiles, which is one contiguous range for each tensor it
- * meets; four 16-byte loads a thread in flight. */
-template <typename G>
+ * meets; two 16-byte loads a thread in flight.  kStream: past the caches, for a long
+ * list that nothing reads again at once (300M bf16: 94 us instead of 106); in front of an update the gradients are left in the last-level
+ * cache for it (100M bf16 with master: 52 + 459 us, 33 + 492 past the caches). */
+template <typename G, bool kStream>
 __global__ void __launch_bounds__(kBlock) k_norm_partial(const Entry* __restrict__ table, int n, int64_t n_tiles,
                                                          double* __restrict__ partial) {
-    __shared__ double lds[kBlock];
+    __shared__ double lds[kBlock / 64];
     const int64_t per = n_tiles / gridDim.x, more = n_tiles % gridDim.x, b = blockIdx.x;
     int64_t tile = b * per + (b < more ? b : more);
     const int64_t end = tile + per + (b < more ? 1 : 0);
@@ -165,7 +183,7 @@ __global__ void __launch_bounds__(kBlock) k_norm_partial(const Entry* __restrict
         const int64_t last = e.first_tile + tiles < end ? e.first_tile + tiles : end;
         if (e.data && last > tile) {
             const int64_t to = (last - e.first_tile) * kTile;
-            sum += sum_squares(static_cast<const G*>(e.data), (tile - e.first_tile) * kTile, to < e.count ? to : e.count, threadIdx.x,
+            sum += sum_squares<G, kStream>(static_cast<const G*>(e.data), (tile - e.first_tile) * kTile, to < e.count ? to : e.count, threadIdx.x,
                                kBlock);
         }
         if (last > tile) tile = last;
@@ -224,7 +242,7 @@ __device__ __forceinline__ double join_partials(const double* partial, int n, do
 
 __global__ void __launch_bounds__(kBlock) k_norm_join(const double* __restrict__ partial, int n, double scale,
                                                       float* __restrict__ norm) {
-    __shared__ double lds[kBlock];
+    __shared__ double lds[kBlock / 64];
     const double total = join_partials(partial, n, lds);
     if (threadIdx.x == 0) norm[0] = (float)(scale * sqrt(total));
 }
@@ -253,7 +271,7 @@ __device__ __forceinline__ bool step_values(const StepArgs& a, float norm, int t
 
 /* one block before the update: the norm (joined from n_partial sums, or given), clipping, bias corrections, the step counter */
 __global__ void __launch_bounds__(kBlock) k_adamw_begin(const StepArgs a) {
-    __shared__ double lds[kBlock];
+    __shared__ double lds[kBlock / 64];
     float norm = 0.0f;
     if (a.n_partial > 0) {
         norm = (float)(fabs(a.grad_scale) * sqrt(join_partials(a.partial, a.n_partial, lds)));
@@ -292,35 +310,45 @@ __device__ __forceinline__ uint32_t max_over_8(uint32_t v) {
     return v;
 }
 
+/* y rounded by dither into byte j of `codes` */
+__device__ __forceinline__ uint32_t put_code(float y, uint32_t dither, uint32_t codes, int j) {
+    return (uint32_t)(j == 0   ? __builtin_amdgcn_cvt_sr_fp8_f32(y, (int)dither, (int)codes, 0)
+                      : j == 1 ? __builtin_amdgcn_cvt_sr_fp8_f32(y, (int)dither, (int)codes, 1)
+                      : j == 2 ? __builtin_amdgcn_cvt_sr_fp8_f32(y, (int)dither, (int)codes, 2)
+                               : __builtin_amdgcn_cvt_sr_fp8_f32(y, (int)dither, (int)codes, 3));
+}
+
 __device__ __forceinline__ float adamw(float w, float& m, float& v, float& root, float g, const StepArgs& a, const Control& c) {
     m = m * a.b1 + g * a.one_minus_b1;
     v = v * a.b2 + g * g * a.one_minus_b2;
-    root = __builtin_sqrtf(v);
-    return w * c.decay - c.step_size * (m / (root * c.inv_root_2 + a.eps));
+    root = __builtin_amdgcn_sqrtf(v); /* root and reciprocal to one unit in the last place: the correctly rounded ones take ten times the
+                                         operations, which bound the 8-bit step */
+    return w * c.decay - c.step_size * (m * __builtin_amdgcn_rcpf(root * c.inv_root_2 + a.eps));
 }
 
 /* a quad's loads and stores; kWhole: all four elements exist, else `count` of them do (tail of a tensor) */
-template <typename T, bool kWhole>
+template <typename T, bool kWhole, bool kStream>
 __device__ __forceinline__ void load_quad(const T* p, int count, float* out) {
     if (kWhole) {
         Quad<T> q;
-        q.load(p);
+        q.template load<kStream>(p);
         _Pragma("unroll") for (int j = 0; j < kVec; ++j) out[j] = q.get(j);
     } else {
         _Pragma("unroll") for (int j = 0; j < kVec; ++j) out[j] = j < count ? to_float(p[j]) : 0.0f;
     }
 }
-template <typename T, bool kWhole>
+template <typename T, bool kWhole, bool kStream>
 __device__ __forceinline__ void store_quad(T* p, int count, const float* v) {
-    if (kWhole) Quad<T>::store(p, v);
+    if (kWhole) Quad<T>::template store<kStream>(p, v);
     else _Pragma("unroll") for (int j = 0; j < kVec; ++j) if (j < count) put(p + j, v[j]);
 }
 
-/* One tile by kThreads threads: kTile / (kThreads * kVec) quads a thread, every load of them issued before the first is used. */
-template <typename P, typename G, bool kBytes, bool kWhole, int kThreads>
+/* One tile by kThreads threads: kTile / (kThreads * kVec) quads a thread, every load of them issued before the first is used (two at a time
+ * with byte codes: their arithmetic, 57 operations an element, wants more waves rather than more loads; 64M bf16 167 us, 175 with four). */
+template <typename P, typename G, bool kBytes, bool kWhole, int kThreads, bool kStream>
 __device__ __forceinline__ void step_tile(const StepArgs& a, const Control& c, P* __restrict__ param, const G* __restrict__ grad,
                                           int64_t state_at, int count) {
-    constexpr int kStep = kThreads * kVec, kUnroll = kWhole ? kTile / kStep : 1;
+    constexpr int kStep = kThreads * kVec, kMost = kTile / kStep, kUnroll = !kWhole ? 1 : kBytes && kMost > 2 ? 2 : kMost;
     const bool master = a.master != nullptr;
     for (int i0 = 0; i0 < (kWhole ? kTile : count); i0 += kUnroll * kStep) {
         float g[kUnroll][kVec], w[kUnroll][kVec], m[kUnroll][kVec], v[kUnroll][kVec];
@@ -328,9 +356,9 @@ __device__ __forceinline__ void step_tile(const StepArgs& a, const Control& c, P
         _Pragma("unroll") for (int u = 0; u < kUnroll; ++u) {
             const int i = i0 + u * kStep + (int)threadIdx.x * kVec, left = count - i;
             const int64_t k = state_at + i;
-            load_quad<G, kWhole>(grad + i, left, g[u]);
-            if (master) load_quad<float, kWhole>(a.master + k, left, w[u]);
-            else load_quad<P, kWhole>(param + i, left, w[u]);
+            load_quad<G, kWhole, kStream>(grad + i, left, g[u]);
+            if (master) load_quad<float, kWhole, kStream>(a.master + k, left, w[u]);
+            else load_quad<P, kWhole, kStream>(param + i, left, w[u]);
             if (kBytes) { /* codes come in whole blocks: the state is padded, the blocks' zeros behind a tensor stay zeros */
                 mc[u] = vc[u] = me[u] = ve[u] = 0;
                 if (kWhole || left > 0) {
@@ -339,8 +367,8 @@ __device__ __forceinline__ void step_tile(const StepArgs& a, const Control& c, P
                     me[u] = a.m_exp[k / kGroup], ve[u] = a.v_exp[k / kGroup];
                 }
             } else {
-                load_quad<float, kWhole>(static_cast<const float*>(a.m) + k, left, m[u]);
-                load_quad<float, kWhole>(static_cast<const float*>(a.v) + k, left, v[u]);
+                load_quad<float, kWhole, kStream>(static_cast<const float*>(a.m) + k, left, m[u]);
+                load_quad<float, kWhole, kStream>(static_cast<const float*>(a.v) + k, left, v[u]);
             }
         }
         _Pragma("unroll") for (int u = 0; u < kUnroll; ++u) {
@@ -365,17 +393,20 @@ __device__ __forceinline__ void step_tile(const StepArgs& a, const Control& c, P
                 }
                 me[u] = block_exponent(max_over_8(most_m)), ve[u] = block_exponent(max_over_8(most_v));
                 const float sm = __uint_as_float((254u - me[u]) << 23), sv = __uint_as_float((254u - ve[u]) << 23);
-                const bool nan_m = me[u] == 255u, nan_v = ve[u] == 255u;
-                uint32_t x = (uint32_t)k * 0x9E3779B1u + c.key;
+                const uint32_t x = (uint32_t)k * 0x9E3779B1u + c.key;
                 mc[u] = vc[u] = 0;
                 _Pragma("unroll") for (int j = 0; j < kVec; ++j) {
                     const uint32_t r = mix(x + j * 0x9E3779B1u);
-                    uint32_t cm = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(m[u][j] * sm, (int)(r & 0xffff0000u), 0, 0) & 0xffu;
-                    uint32_t cv = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(root[j] * sv, (int)(r << 16), 0, 0) & 0xffu;
-                    if (cv == 0 && root[j] > 0.0f) cv = 1;
-                    if (nan_m) cm = 0x7f;
-                    if (nan_v) cv = 0x7f;
-                    if (kWhole || j < left) mc[u] |= cm << (8 * j), vc[u] |= cv << (8 * j);
+                    /* a root that is not 0 keeps the smallest code: 2^-9 and any dither give it */
+                    const float y = root[j] > 0.0f ? fmaxf(root[j] * sv, 0x1p-9f) : 0.0f;
+                    mc[u] = put_code(m[u][j] * sm, r & 0xffff0000u, mc[u], j);
+                    vc[u] = put_code(y, r << 16, vc[u], j);
+                }
+                if (me[u] == 255u) mc[u] = 0x7f7f7f7fu; /* a block with an infinity or NaN is NaN */
+                if (ve[u] == 255u) vc[u] = 0x7f7f7f7fu;
+                if (!kWhole) { /* codes behind the tensor's end stay zeros */
+                    const uint32_t keep = left >= 4 ? ~0u : left > 0 ? (1u << (8 * left)) - 1u : 0u;
+                    mc[u] &= keep, vc[u] &= keep;
                 }
                 if (kWhole || left > 0) {
                     *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + k) = mc[u];
@@ -383,16 +414,19 @@ __device__ __forceinline__ void step_tile(const StepArgs& a, const Control& c, P
                     if (k % kGroup == 0) a.m_exp[k / kGroup] = (uint8_t)me[u], a.v_exp[k / kGroup] = (uint8_t)ve[u];
                 }
             } else {
-                store_quad<float, kWhole>(static_cast<float*>(a.m) + k, left, m[u]);
-                store_quad<float, kWhole>(static_cast<float*>(a.v) + k, left, v[u]);
+                store_quad<float, kWhole, kStream>(static_cast<float*>(a.m) + k, left, m[u]);
+                store_quad<float, kWhole, kStream>(static_cast<float*>(a.v) + k, left, v[u]);
             }
-            store_quad<P, kWhole>(param + i, left, w[u]);
-            if (master) store_quad<float, kWhole>(a.master + k, left, w[u]);
+            store_quad<P, kWhole, kStream>(param + i, left, w[u]);
+            if (master) store_quad<float, kWhole, kStream>(a.master + k, left, w[u]);
         }
     }
 }
 
-template <typename P, typename G, bool kBytes>
+/* kStream: everything but the byte codes past the caches.  For lists whose arrays do not fit the 256 MiB last-level cache together, where
+ * what a step leaves there only pushes out what it still has to read: 100M bf16 + fp32 master 500 -> 452 us (and the norm in front of
+ * it 71 -> 37); 16M fp32, which fits, 70 us without and 80 with. */
+template <typename P, typename G, bool kBytes, bool kStream>
 __global__ void __launch_bounds__(kBlock) k_adamw(const StepArgs a) {
     const Control c = *a.control;
     if (c.skip) return;
@@ -403,8 +437,8 @@ __global__ void __launch_bounds__(kBlock) k_adamw(const StepArgs a) {
         if (!e.data || !grad) continue;
         const int64_t from = (tile - e.first_tile) * kTile;
         P* param = static_cast<P*>(e.data) + from;
-        if (e.count - from >= kTile) step_tile<P, G, kBytes, true, kBlock>(a, c, param, grad + from, e.state_at + from, kTile);
-        else step_tile<P, G, kBytes, false, kBlock>(a, c, param, grad + from, e.state_at + from, (int)(e.count - from));
+        if (e.count - from >= kTile) step_tile<P, G, kBytes, true, kBlock, kStream>(a, c, param, grad + from, e.state_at + from, kTile);
+        else step_tile<P, G, kBytes, false, kBlock, kStream>(a, c, param, grad + from, e.state_at + from, (int)(e.count - from));
     }
 }
 
@@ -421,7 +455,7 @@ __global__ void __launch_bounds__(kSmallBlock) k_adamw_small(const StepArgs a, i
         if (wave < a.n_tiles) {
             const Entry e = a.grads[find_tensor(a.grads, a.n, wave)];
             const int64_t from = (wave - e.first_tile) * kTile, to = from + kTile;
-            if (e.data) sum = sum_squares(static_cast<const G*>(e.data), from, to < e.count ? to : e.count, threadIdx.x & 63, 64);
+            if (e.data) sum = sum_squares<G, false>(static_cast<const G*>(e.data), from, to < e.count ? to : e.count, threadIdx.x & 63, 64);
         }
         for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
         if ((threadIdx.x & 63) == 0) lds[wave] = sum;
@@ -456,17 +490,24 @@ __global__ void __launch_bounds__(kSmallBlock) k_adamw_small(const StepArgs a, i
     if (!e.data || !grad) return;
     const int64_t from = (blockIdx.x - e.first_tile) * kTile;
     P* param = static_cast<P*>(e.data) + from;
-    if (e.count - from >= kTile) step_tile<P, G, kBytes, true, kSmallBlock>(a, c, param, grad + from, e.state_at + from, kTile);
-    else step_tile<P, G, kBytes, false, kSmallBlock>(a, c, param, grad + from, e.state_at + from, (int)(e.count - from));
+    if (e.count - from >= kTile) step_tile<P, G, kBytes, true, kSmallBlock, false>(a, c, param, grad + from, e.state_at + from, kTile);
+    else step_tile<P, G, kBytes, false, kSmallBlock, false>(a, c, param, grad + from, e.state_at + from, (int)(e.count - from));
 }
 
 int norm_blocks(int64_t n_tiles) { return (int)(n_tiles < kMaxPartials ? n_tiles : kMaxPartials); }
 
-void launch_norm(const Entry* table, int n, int64_t n_tiles, int dtype, double* partial, hipStream_t st) {
+template <typename G>
+void launch_norm(const Entry* table, int n, int64_t n_tiles, bool stream, double* partial, hipStream_t st) {
     const dim3 grid((unsigned)norm_blocks(n_tiles)), block(kBlock);
-    if (dtype == MZS_DTYPE_FLOAT) hipLaunchKernelGGL(k_norm_partial<float>, grid, block, 0, st, table, n, n_tiles, partial);
-    else if (dtype == MZS_DTYPE_BFLOAT) hipLaunchKernelGGL(k_norm_partial<bf16>, grid, block, 0, st, table, n, n_tiles, partial);
-    else hipLaunchKernelGGL(k_norm_partial<_Float16>, grid, block, 0, st, table, n, n_tiles, partial);
+    if (stream) hipLaunchKernelGGL((k_norm_partial<G, true>), grid, block, 0, st, table, n, n_tiles, partial);
+    else hipLaunchKernelGGL((k_norm_partial<G, false>), grid, block, 0, st, table, n, n_tiles, partial);
+}
+constexpr double kCache = 256.0 * 1048576.0; /* bytes of the last-level cache */
+void launch_norm(const Entry* table, int n, int64_t n_tiles, int dtype, bool alone, double* partial, hipStream_t st) {
+    const bool stream = alone && (double)n_tiles * kTile * (dtype == MZS_DTYPE_FLOAT ? 4 : 2) > kCache;
+    if (dtype == MZS_DTYPE_FLOAT) launch_norm<float>(table, n, n_tiles, stream, partial, st);
+    else if (dtype == MZS_DTYPE_BFLOAT) launch_norm<bf16>(table, n, n_tiles, stream, partial, st);
+    else launch_norm<_Float16>(table, n, n_tiles, stream, partial, st);
 }
 
 struct Launch {
@@ -483,8 +524,12 @@ void launch_step(const Launch& l) {
         return;
     }
     const dim3 grid((unsigned)(l.s.n_tiles < 65536 ? l.s.n_tiles : 65536)), block(kBlock);
-    if (l.bits == 8) hipLaunchKernelGGL((k_adamw<P, G, true>), grid, block, 0, l.st, l.s);
-    else hipLaunchKernelGGL((k_adamw<P, G, false>), grid, block, 0, l.st, l.s);
+    const double each = sizeof(P) + sizeof(G) + (l.s.master ? 4 : 0) + (l.bits == 8 ? 2.0625 : 8.0);
+    const bool stream = each * kTile * (double)l.s.n_tiles > kCache;
+    if (l.bits == 8 && stream) hipLaunchKernelGGL((k_adamw<P, G, true, true>), grid, block, 0, l.st, l.s);
+    else if (l.bits == 8) hipLaunchKernelGGL((k_adamw<P, G, true, false>), grid, block, 0, l.st, l.s);
+    else if (stream) hipLaunchKernelGGL((k_adamw<P, G, false, true>), grid, block, 0, l.st, l.s);
+    else hipLaunchKernelGGL((k_adamw<P, G, false, false>), grid, block, 0, l.st, l.s);
 }
 template <typename P>
 void launch_step(const Launch& l, int grad_dtype) {
@@ -543,7 +588,7 @@ int mzs_grad_norm(int32_t device, int32_t n, const void* table_dev, int64_t n_ti
     if (scope.status != hipSuccess) return hip_error("mzs_grad_norm: device", scope.status);
     hipStream_t st = static_cast<hipStream_t>(stream);
     double* partial = static_cast<double*>(workspace);
-    if (n_tiles > 0) launch_norm(static_cast<const Entry*>(table_dev), n, n_tiles, dtype, partial, st);
+    if (n_tiles > 0) launch_norm(static_cast<const Entry*>(table_dev), n, n_tiles, dtype, true, partial, st);
     hipLaunchKernelGGL(k_norm_join, dim3(1), dim3(kBlock), 0, st, (const double*)partial, n_tiles > 0 ? norm_blocks(n_tiles) : 0,
                        std::fabs(grad_scale), norm_dev);
     const hipError_t e = hipGetLastError();
@@ -587,7 +632,7 @@ int mzs_adamw_step(const mzs_adamw_args* a, void* stream) {
     if (!small) {
         if (compute) {
             s.n_partial = norm_blocks(a->n_tiles);
-            launch_norm(s.grads, a->n, a->n_tiles, a->grad_dtype, static_cast<double*>(a->workspace), st);
+            launch_norm(s.grads, a->n, a->n_tiles, a->grad_dtype, false, static_cast<double*>(a->workspace), st);
         }
         hipLaunchKernelGGL(k_adamw_begin, dim3(1), dim3(kBlock), 0, st, s);
     }

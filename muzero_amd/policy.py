@@ -113,11 +113,11 @@ def _run(name, logits, actions, mask, temperature, top, saved=None, upstream=Non
     lp = h = z = st = tl = ta = 0
     if saved is None:
         if apart:       # autograd's outputs are no views of one tensor
-            log_prob, entropy, log_z, stats = (torch.empty(s, dtype=torch.float32, device=device)
+            log_prob, entropy, log_z, stats = (logits.new_empty(s, dtype=torch.float32)
                                                for s in (shape[:-1], shape[:-1], shape[:-1], (rows, 2)))
             lp, h, z, st = log_prob.data_ptr(), entropy.data_ptr(), log_z.data_ptr(), stats.data_ptr()
         else:
-            flat = torch.empty((5, rows), dtype=torch.float32, device=device)
+            flat = logits.new_empty((5, rows), dtype=torch.float32)
             log_prob, entropy, log_z, _, _ = flat.unbind()
             lp = flat.data_ptr()
             h, z, st = lp + 4 * rows, lp + 8 * rows, lp + 12 * rows
@@ -125,8 +125,8 @@ def _run(name, logits, actions, mask, temperature, top, saved=None, upstream=Non
                 lead = shape[:-1]
                 log_prob, entropy, log_z = log_prob.view(lead), entropy.view(lead), log_z.view(lead)
         if top:
-            top_lp = torch.empty(shape[:-1] + (top,), dtype=torch.float32, device=device)
-            top_at = torch.empty(shape[:-1] + (top,), dtype=torch.int32, device=device)
+            top_lp = logits.new_empty((*shape[:-1], top), dtype=torch.float32)
+            top_at = logits.new_empty((*shape[:-1], top), dtype=torch.int32)
             tl, ta = top_lp.data_ptr(), top_at.data_ptr()
         values = PolicyLogProbs(log_prob, entropy, log_z, top_lp, top_at)
     else:
@@ -134,7 +134,7 @@ def _run(name, logits, actions, mask, temperature, top, saved=None, upstream=Non
     g_lp = g_h = g_z = g = g_pitch = 0
     if upstream is not None:
         g_lp, g_h, g_z = (0 if u is None else u.data_ptr() for u in upstream)
-        grad = torch.empty(shape, dtype=logits.dtype, device=device) if out is None else out
+        grad = logits.new_empty(shape) if out is None else out
         g, g_pitch = grad.data_ptr(), (grad.stride(0) if dim == 2 else n)
     if rows:
         args = [device.index, _DTYPES[logits.dtype], rows, n, rows_of.data_ptr(), pitch, mask_ptr, mask_pitch, action_ptr, action_bytes,
