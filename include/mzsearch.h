@@ -191,6 +191,7 @@ int mzs_prediction_inference(mzs_handle* h, int32_t batch, const float* hidden_d
  * mzs_set_weights and every mzs_train_apply refreshes what the search / inference kernels read. */
 #define MZS_OPT_ADAM 0 /* torch.optim.Adam(lr, betas 0.9/0.999, eps 1e-8), muzero_model.py:419 */
 #define MZS_OPT_SGD 1  /* torch.optim.SGD(lr, momentum 0.9), muzero_model.py:421               */
+#define MZS_OPT_ADAMW 2 /* decoupled weight decay, optional clipping (mzs_train_set_adamw); no counterpart in the reference */
 
 /* Allocates the per-sample tapes for batches of up to max_batch samples (this rank's shard) and
  * k_hypothetical_steps = unroll_steps (muzero_model.py:623), and zeroed optimizer state. */
@@ -267,6 +268,11 @@ int mzs_train_set_loss(mzs_handle* h, int32_t value_criterion, int32_t reward_cr
  * muzero_model.py:418-421 constructs).  OneCycleLR (muzero_model.py:433) cycles it per step together
  * with the rate: the caller evaluates both on the host (muzero_amd/train.py) and passes them in. */
 int mzs_train_set_momentum(mzs_handle* h, double momentum);
+
+/* What MZS_OPT_ADAMW steps with (mzs_adamw_step on the weights, fp32 states of their own in the handle): beta1 is
+ * mzs_train_set_momentum's; max_norm > 0 clips the gradient's global norm (the running statistics' slots of the vision model not
+ * among it) and skips a step whose norm is not finite.  Allocates on the first call, later ones change the values. */
+int mzs_train_set_adamw(mzs_handle* h, double beta2, double eps, double weight_decay, double max_norm);
 
 /* optimizer.step() (muzero_model.py:764) with the (all-reduced) gradient; lr is the scheduler's
  * current value (muzero_amd/train.py evaluates the reference's schedulers on the host). */
@@ -416,7 +422,7 @@ int mzs_replay_update_value(int32_t batch, int32_t num_unroll, double* const* ro
  * A row that allows nothing (all masked or -inf): log_z = log_prob = -inf, entropy 0, gradient 0, no alternatives.
  * Action < 0: the row has none (log_prob 0, g_a not used).  Action >= n_actions: log_prob NaN.  Action forbidden:
  * log_prob -inf, and its own gradient element stays 0.  A NaN or +inf among the allowed logits makes the row's values and
- * gradient NaN (alternatives: NaN ranks first); masked logits are never looked at.  Slots of alternatives beyond the allowed
+ * gradient NaN (alternatives: NaN ranks first), forbidden actions' gradient is 0 there too; masked logits are never looked at.  Slots of alternatives beyond the allowed
  * actions hold index -1 and -inf.
  * Everything is computed in fp32; logits and gradient are fp32, bf16 or fp16. */
 #define MZS_DTYPE_FLOAT 0
@@ -473,6 +479,7 @@ int mzs_policy_log_probs_train(const mzs_policy_args* args, void* stream);
 #define MZS_OPTIM_BLOCK 32       /* 8-bit states: elements that share one exponent                          */
 #define MZS_OPTIM_ENTRY_BYTES 32 /* device table: bytes per tensor (one more entry behind the last)         */
 #define MZS_OPTIM_CONTROL_BYTES 64
+#define MZS_OPTIM_CONTROL_SKIP 3
 
 /* Writes the table of n tensors to table_dev ((n + 1) * MZS_OPTIM_ENTRY_BYTES bytes, 16-byte aligned): tensor i has counts[i]
  * elements from pointers[i] on (device memory, contiguous; NULL: no tensor — a parameter without a gradient).
@@ -513,7 +520,8 @@ typedef struct mzs_adamw_args {
     void* exp_avg_sq;                /* fp32 v, or the e4m3 codes of its root                          */
     uint8_t* exp_avg_exponent;       /* state_bits 8: e8m0 bytes, one per 32 elements                  */
     uint8_t* exp_avg_sq_exponent;
-    int32_t* control_dev;            /* MZS_OPTIM_CONTROL_BYTES: [0] steps taken, [1] steps skipped; the rest is the step's own */
+    int32_t* control_dev;            /* MZS_OPTIM_CONTROL_BYTES, zeros at first: [0] steps taken, [1] steps skipped,
+                                        [MZS_OPTIM_CONTROL_SKIP] 1 if the last one was; the rest is the step's own */
     float* norm_dev;                 /* the norm (written unless norm_given); may be NULL without max_norm */
     const float* lr_dev;             /* or NULL: lr                                                    */
     double lr, beta1, beta2, eps, weight_decay, max_norm, grad_scale;

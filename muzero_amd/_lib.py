@@ -14,7 +14,7 @@ LIB_PATH = os.environ.get("MZS_LIB") or os.path.join(_HERE, "libmzsearch.so")
 
 ENGINE_FUSED = 0
 ENGINE_FUSED_GENERIC = 2
-OPT_ADAM, OPT_SGD = 0, 1
+OPT_ADAM, OPT_SGD, OPT_ADAMW = 0, 1, 2
 
 TREE_VISIT, TREE_VALUE_SUM, TREE_PRIOR, TREE_REWARD, TREE_CHILD_BASE = 0, 1, 2, 3, 4
 TREE_SIM_LEAF, TREE_MINMAX, TREE_HIDDEN, TREE_STATUS = 5, 6, 7, 8
@@ -117,6 +117,7 @@ _SIGNATURES = {
     "mzs_train_set_loss": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32]),
     "mzs_train_set_momentum": (C.c_int, [C.c_void_p, C.c_double]),
     "mzs_train_apply": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_double, C.c_void_p]),
+    "mzs_train_set_adamw": (C.c_int, [C.c_void_p, C.c_double, C.c_double, C.c_double, C.c_double]),
     "mzs_train_dropout_count": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(C.c_int64)]),
     "mzs_train_set_dropout": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_uint64]),
     "mzs_get_weights": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t]),

@@ -7,6 +7,9 @@ optional extra section, `mi355x`, for the batched engine:
 
     "mi355x": {"concurrent_games": 4096, "num_gpus": 8, "engine": "fused"}
 
+`muzero.optimizer` may also be "adamw"; its weight_decay and max_grad_norm stand in the extra section as
+"optimizer_options": {"weight_decay": 0.01, "max_grad_norm": 1.0}.
+
 Reference configs (no `mi355x` section) load with the defaults below.
 """
 import json

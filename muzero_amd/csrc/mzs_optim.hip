@@ -7,6 +7,7 @@
 #include "mzs_error.h"
 
 #include <cmath>
+#include <cstddef>
 #include <cstdint>
 #include <cstring>
 
@@ -203,7 +204,7 @@ struct Control {
     float decay;        /* 1 - lr * weight_decay              */
     float inv_root_2;   /* 1 / sqrt(1 - beta2^t)              */
 };
-static_assert(sizeof(Control) <= MZS_OPTIM_CONTROL_BYTES, "control size");
+static_assert(sizeof(Control) <= MZS_OPTIM_CONTROL_BYTES && offsetof(Control, skip) == 4 * MZS_OPTIM_CONTROL_SKIP, "control layout");
 
 struct StepArgs {
     const Entry* params;
@@ -478,6 +479,7 @@ __global__ void __launch_bounds__(kSmallBlock) k_adamw_small(const StepArgs a, i
             if (go) a.control->step = t;
             else a.control->skipped += 1;
             if (norm_here && a.norm) a.norm[0] = norm;
+            a.control->skip = c.skip;
             a.control->ticket = 0;
         }
     }

@@ -475,6 +475,22 @@ __global__ void __launch_bounds__(256) k_train_apply(const ApplyParams p) {
     if (p.store16) p.store16[so] = ((si >> 30) & 1) ? w : mzs_bf16_round(w);
 }
 
+/* after an AdamW step of the blob: running statistics move, the store the search kernels read follows (as in k_train_apply); nothing
+ * where the step was skipped */
+__global__ void __launch_bounds__(256) k_train_refresh(float* __restrict__ blob, float* __restrict__ store, float* __restrict__ store16,
+                                                       const int* __restrict__ store_index, const unsigned char* __restrict__ is_stat,
+                                                       const float* __restrict__ grad, int n, const int* __restrict__ skip) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n || *skip) return;
+    if (is_stat && is_stat[i]) blob[i] += grad[i];
+    if (!store_index) return;
+    const int si = store_index[i], so = si & 0x3fffffff;
+    if (si == -1) return;
+    const float w = blob[i];
+    store[so] = w;
+    if (store16) store16[so] = ((si >> 30) & 1) ? w : mzs_bf16_round(w);
+}
+
 /* vision_model: the Linear layers' stores (quads for mzs_vision.h, [K/4][N_pad][4] for mzs_vision_mm.h) are
  * permutations of blob elements with zero padding: src[i] = blob index or -1 */
 __global__ void __launch_bounds__(256) k_vis_store_refresh(float* __restrict__ store, const int* __restrict__ src,

@@ -660,6 +660,12 @@ struct mzs_handle {
     uint64_t dropout_seed = 0x5DEECE66Dull, train_calls = 0;
     int loss_value = MZS_LOSS_CE, loss_reward = MZS_LOSS_CE; /* mzs_train_set_loss */
     double momentum = 0.9;                                   /* mzs_train_set_momentum */
+    /* mzs_train_set_adamw: one optimizer tensor for each run of blob elements that are optimised (all of them but the vision model's
+     * running statistics), states and tables as mzs_adamw_step takes them */
+    mzs_adamw_args adamw = {};                               /* n = 0: not set */
+    std::vector<int64_t> adamw_start, adamw_count;
+    std::vector<const void*> adamw_grads;
+    void* adamw_grad_table = nullptr;
     size_t w_floats = 0;
     bool have_weights = false;
     int n_nodes_max = 0;
@@ -2233,33 +2239,115 @@ int mzs_train_set_momentum(mzs_handle* h, double momentum) {
     return MZS_OK;
 }
 
+int mzs_train_set_adamw(mzs_handle* h, double beta2, double eps, double weight_decay, double max_norm) {
+    if (!h) return fail(MZS_E_ARG, "null handle");
+    if (!h->tape_dev && !h->vis_train) return fail(MZS_E_STATE, "mzs_train_create has not been called");
+    if (!(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0 && weight_decay >= 0.0 && max_norm >= 0.0) ||
+        !std::isfinite(eps + weight_decay + max_norm))
+        return fail(MZS_E_ARG, "beta2 must be in [0, 1), eps, weight_decay and max_norm finite and not negative");
+    HIP_TRY(hipSetDevice(h->cfg.device));
+    mzs_adamw_args& a = h->adamw;
+    if (a.n == 0) {
+        const int64_t total = (int64_t)mzs_blob_total(&h->cfg.dims);
+        std::vector<unsigned char> is_stat((size_t)total, 0);
+        if (h->vis_train)
+            HIP_TRY(hipMemcpy(is_stat.data(), vis_train_stat_flags(h->vis_train), (size_t)total, hipMemcpyDeviceToHost));
+        std::vector<int64_t> start, count;
+        int64_t padded = 0;
+        for (int64_t i = 0; i < total;) {
+            int64_t j = i;
+            while (j < total && !is_stat[(size_t)j]) ++j;
+            if (j > i) {
+                start.push_back(i), count.push_back(j - i);
+                padded += (j - i + MZS_OPTIM_ALIGN - 1) / MZS_OPTIM_ALIGN * MZS_OPTIM_ALIGN;
+            }
+            i = j + 1;
+        }
+        const size_t table = (start.size() + 1) * MZS_OPTIM_ENTRY_BYTES;
+        unsigned char *params = nullptr, *grads = nullptr, *work = nullptr, *control = nullptr;
+        float *m = nullptr, *v = nullptr, *norm = nullptr;
+        std::vector<const void*> at(start.size());
+        for (size_t k = 0; k < at.size(); ++k) at[k] = h->blob_dev + start[k];
+        int rc;
+        int64_t tiles = 0;
+        if ((rc = dev_alloc(h, &params, table)) || (rc = dev_alloc(h, &grads, table)) || (rc = dev_alloc(h, &m, (size_t)padded)) ||
+            (rc = dev_alloc(h, &v, (size_t)padded)) || (rc = dev_alloc(h, &control, MZS_OPTIM_CONTROL_BYTES)) ||
+            (rc = dev_alloc(h, &norm, 1)) ||
+            (rc = mzs_optim_table(h->cfg.device, (int32_t)start.size(), at.data(), count.data(), params, &tiles, nullptr)))
+            return rc;
+        const size_t bytes = mzs_grad_norm_workspace(tiles);
+        if ((rc = dev_alloc(h, &work, bytes))) return rc;
+        HIP_TRY(hipDeviceSynchronize()); /* the table was written on the null stream */
+        a.device = h->cfg.device;
+        a.n_tiles = tiles;
+        a.param_dtype = a.grad_dtype = MZS_DTYPE_FLOAT;
+        a.state_bits = 32;
+        a.params_table = params, a.grads_table = grads;
+        a.exp_avg = m, a.exp_avg_sq = v;
+        a.control_dev = reinterpret_cast<int32_t*>(control);
+        a.norm_dev = norm;
+        a.workspace = work, a.workspace_bytes = bytes;
+        a.grad_scale = 1.0;
+        h->adamw_start = start, h->adamw_count = count;
+        h->adamw_grads.resize(start.size());
+        a.n = (int32_t)start.size();
+    }
+    a.beta2 = beta2, a.eps = eps, a.weight_decay = weight_decay, a.max_norm = max_norm;
+    return MZS_OK;
+}
+
+static int train_apply_adamw(mzs_handle* h, const float* grad_dev, double lr, hipStream_t st) {
+    mzs_adamw_args& a = h->adamw;
+    if (a.n == 0) return fail(MZS_E_STATE, "mzs_train_set_adamw has not been called");
+    HIP_TRY(hipSetDevice(h->cfg.device));
+    for (size_t k = 0; k < h->adamw_grads.size(); ++k) h->adamw_grads[k] = grad_dev + h->adamw_start[k];
+    int64_t tiles = 0;
+    int rc = mzs_optim_table(a.device, a.n, h->adamw_grads.data(), h->adamw_count.data(), const_cast<void*>(a.grads_table), &tiles, st);
+    if (rc) return rc;
+    a.lr = lr, a.beta1 = h->momentum;
+    if ((rc = mzs_adamw_step(&a, st))) return rc;
+    const int n = (int)mzs_blob_total(&h->cfg.dims);
+    hipLaunchKernelGGL(k_train_refresh, dim3((n + 255) / 256), dim3(256), 0, st, h->blob_dev, h->w_dev,
+                       h->w_search_dev != h->w_dev ? h->w_search_dev : (float*)nullptr,
+                       h->vis_train ? (const int*)nullptr : (const int*)h->store_index_dev,
+                       h->vis_train ? vis_train_stat_flags(h->vis_train) : (const unsigned char*)nullptr, grad_dev, n,
+                       (const int*)a.control_dev + MZS_OPTIM_CONTROL_SKIP);
+    HIP_TRY(hipGetLastError());
+    return MZS_OK;
+}
+
 int mzs_train_apply(mzs_handle* h, const float* grad_dev, int32_t optimizer, double lr, void* stream) {
     if (!h || !grad_dev) return fail(MZS_E_ARG, "null argument");
     if (!h->tape_dev && !h->vis_train) return fail(MZS_E_STATE, "mzs_train_create has not been called");
     if (!h->have_weights) return fail(MZS_E_STATE, "mzs_set_weights has not been called");
-    if (optimizer != MZS_OPT_ADAM && optimizer != MZS_OPT_SGD) return fail(MZS_E_ARG, "unknown optimizer");
+    if (optimizer != MZS_OPT_ADAM && optimizer != MZS_OPT_SGD && optimizer != MZS_OPT_ADAMW) return fail(MZS_E_ARG, "unknown optimizer");
     HIP_TRY(hipSetDevice(h->cfg.device));
-    h->train_step += 1;
     ApplyParams p;
-    p.blob = h->blob_dev;
-    p.store = h->w_dev;
-    p.store16 = h->w_search_dev != h->w_dev ? h->w_search_dev : nullptr;
-    p.store_index = h->vis_train ? nullptr : h->store_index_dev;
-    p.is_stat = h->vis_train ? vis_train_stat_flags(h->vis_train) : nullptr;
-    p.m = h->adam_m_dev;
-    p.v = h->adam_v_dev;
-    p.grad = grad_dev;
     p.n = (int)mzs_blob_total(&h->cfg.dims);
-    p.optimizer = optimizer;
-    p.step = h->train_step;
-    const double bc1 = 1.0 - std::pow(h->momentum, h->train_step), bc2 = 1.0 - std::pow(0.999, h->train_step);
-    p.momentum = (float)h->momentum;
-    p.one_minus_momentum = (float)(1.0 - h->momentum);
-    p.lr_over_bc1 = (float)(lr / bc1);
-    p.inv_sqrt_bc2 = (float)(1.0 / std::sqrt(bc2));
-    p.lr = (float)lr;
-    hipLaunchKernelGGL(k_train_apply, dim3((p.n + 255) / 256), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), p);
+    if (optimizer == MZS_OPT_ADAMW) {
+        const int rc = train_apply_adamw(h, grad_dev, lr, static_cast<hipStream_t>(stream));
+        if (rc) return rc;
+    } else {
+        h->train_step += 1;
+        p.blob = h->blob_dev;
+        p.store = h->w_dev;
+        p.store16 = h->w_search_dev != h->w_dev ? h->w_search_dev : nullptr;
+        p.store_index = h->vis_train ? nullptr : h->store_index_dev;
+        p.is_stat = h->vis_train ? vis_train_stat_flags(h->vis_train) : nullptr;
+        p.m = h->adam_m_dev;
+        p.v = h->adam_v_dev;
+        p.grad = grad_dev;
+        p.optimizer = optimizer;
+        p.step = h->train_step;
+        const double bc1 = 1.0 - std::pow(h->momentum, h->train_step), bc2 = 1.0 - std::pow(0.999, h->train_step);
+        p.momentum = (float)h->momentum;
+        p.one_minus_momentum = (float)(1.0 - h->momentum);
+        p.lr_over_bc1 = (float)(lr / bc1);
+        p.inv_sqrt_bc2 = (float)(1.0 / std::sqrt(bc2));
+        p.lr = (float)lr;
+        hipLaunchKernelGGL(k_train_apply, dim3((p.n + 255) / 256), dim3(256), 0,
+                           static_cast<hipStream_t>(stream), p);
+    }
     if (h->vis_train) { /* the Linear layers' stores of the search kernels (mzs_vision.h, mzs_vision_mm.h) */
         const mzs_dims& d = h->cfg.dims;
         const int n_store = (int)(vis_lin_total(d.hidden_dim, d.n_mid_layers, d.state_dim, d.n_actions) +

@@ -248,6 +248,7 @@ class Muzero:
         self.store_loss = []
         self.bin_method, self.bin_decomposition_number = bin_method, bin_decomposition_number
         self.is_RGB = "vision" in self.model_structure       # muzero_model.py:282
+        self.optimizer_options = {}     # weight_decay, max_grad_norm of optimizer="adamw": read by the first train()
         self._engine = None
         self._trainer = None
         self._blob = None
@@ -403,6 +404,18 @@ class Muzero:
         val = val.cpu().numpy()
         return pol.cpu().numpy(), (val if reanalyze else val[0])
 
+    def policy_statistics(self, states, actions=None, temperature=1.0, top=0):
+        """The policy head on a batch of observations as PolicyLogProbs (muzero_amd.policy): the log-probability of
+        `actions` (indices into action_dictionnary; None: 0), the entropy and the `top` most likely actions of
+        softmax(logits / temperature).  No counterpart in the reference (its inference returns the softmax alone,
+        muzero_model.py:883-905)."""
+        from .policy import policy_log_probs
+        obs = self._as_images(states) if self.is_RGB else self._as_batch(states)
+        _, pol, _ = self._inference_engine().initial_inference(obs)
+        if actions is not None:
+            actions = torch.as_tensor(actions).reshape(-1).to(device=pol.device, dtype=torch.int64)
+        return policy_log_probs(torch.log(pol), actions, temperature=temperature, top=top)
+
     def train(self, batch):
         """muzero_model.py:791-811: one optimizer step on `batch` = (samples, importance-sampling
         ratio, game positions) as ReplayBuffer.sample_batch returns it (replay_buffer.py:131-166).
@@ -432,7 +445,7 @@ class Muzero:
                                       "model with the largest batch first")
         if self._trainer is None:
             self._trainer = tr.Trainer(self._inference_engine(), self.k_hypothetical_steps, B, self.opt, self.lr,
-                                       self.sch, self.epoch, self.loss_type)
+                                       self.sch, self.epoch, self.loss_type, **self.optimizer_options)
         t = self._trainer
         t.count = self.count
         prio = t.step(obs, actions, tv, trw, tp, ratio)
@@ -456,7 +469,8 @@ class Muzero:
                 "optimizer": self.opt, "loss_type": self.loss_type, "lr_scheduler": self.sch,
                 "num_of_epoch": self.epoch, "device": self.device, "random_tag": self.random_tag,
                 "action_map": self.action_dictionnary, "model_structure": self.model_structure,
-                "use_amp": self.use_amp, "type_format": str(self.type_format)}
+                "use_amp": self.use_amp, "type_format": str(self.type_format),
+                **({"optimizer_options": self.optimizer_options} if self.optimizer_options else {})}
 
     def save_model(self, directory="model_checkpoint", tag=None, model_update_condition=None):
         """Same JSON as muzero_model.py:923-941; the weights go to one `.npz` blob instead of
@@ -486,6 +500,7 @@ class Muzero:
                    hidden_layer_dimensions=iv["hidden_layer_dimensions"],
                    number_of_hidden_layer=iv["number_of_hidden_layer"], load=True,
                    type_format=torch.bfloat16 if "bfloat16" in str(iv.get("type_format", "")) else torch.float32)
+        self.optimizer_options = dict(iv.get("optimizer_options", {}))
         self.observation_dimension = iv["observation_space_dimensions"]
         self.action_dictionnary = iv["action_map"]
         self.action_dimension = len(self.action_dictionnary)

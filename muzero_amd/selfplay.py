@@ -440,6 +440,19 @@ class Arena:
                                                       self.eng._stream()), "mzs_arena_priority_packed")
         return out
 
+    def policy_statistics(self, row0, n_rows, temperature=1.0, top=0):
+        """What the search recommended in trajectory rows [row0, row0 + n_rows) (the child visit fractions Game.store_search_statistics
+        keeps, game.py:154-168, as a distribution at `temperature`), as PolicyLogProbs [n_rows, max_moves] (muzero_amd.policy):
+        the log-probability of the action that was played, the entropy, the `top` alternatives.  The rows are finished
+        games'; moves a game did not reach: log_prob 0, log_z -inf, entropy 0, no alternatives."""
+        from .policy import policy_log_probs
+        if row0 < 0 or n_rows < 1 or row0 + n_rows > self.n_rows:
+            raise ValueError(f"rows [{row0}, {row0 + n_rows}) out of {self.n_rows}")
+        rows = slice(int(row0), int(row0) + int(n_rows))
+        reached = torch.arange(self.T, device=self.eng.device)[None, :] < self.arrays["length"][rows, None]
+        logits = torch.log(torch.where(reached[:, :, None], self.arrays["policy"][rows], 0.0))
+        return policy_log_probs(logits, torch.where(reached, self.arrays["action"][rows], -1), temperature=temperature, top=top)
+
     def make_batch(self, row_pos, num_unroll, td_steps, discount):
         """ReplayBuffer.sample_batch's gather + Game.make_target on the device, in the layout
         muzero_amd.train.Trainer.grad_step takes: obs [B, obs], actions [K, B, A], target value /
@@ -599,6 +612,7 @@ class SelfPlay:
                     num_of_epoch=m["num_of_epoch"], hidden_layer_dimensions=m["hidden_layer_dimensions"],
                     number_of_hidden_layer=m["number_of_hidden_layer"], bin_method=m["bin_method"],
                     bin_decomposition_number=m["bin_decomposition_number"])
+        mz.optimizer_options = dict(extra.get("optimizer_options", {}))
         if weights is not None:
             mz.set_weights(weights)
         eng = SearchEngine(mz.dims, max_games=G, max_simulations=S, discount=mc["discount"],
@@ -608,7 +622,7 @@ class SelfPlay:
         eng.set_weights(mz.weights_blob())
         mz._engine = eng
         trainer = Trainer(eng, m["k_hypothetical_steps"], rb["batch_size"], m["optimizer"], m["learning_rate"],
-                          m["lr_scheduler"], m["num_of_epoch"], m["loss_type"])
+                          m["lr_scheduler"], m["num_of_epoch"], m["loss_type"], **mz.optimizer_options)
         mz._trainer = trainer
         from .shard import rank_world
         if rank_world()[1] > 1:      # Trainer broadcast rank 0's weights into the handle: mz follows
