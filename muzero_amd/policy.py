@@ -90,6 +90,22 @@ def _coefficient(g, name, lead, device):
     return g if g.dtype is torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()
 
 
+def _overlap(out, logits):
+    """Whether the two share elements without being the same view (columns of one wide buffer are apart)."""
+    if out.untyped_storage().data_ptr() != logits.untyped_storage().data_ptr() or not out.numel():
+        return False
+    if out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride():
+        return False
+    reach = lambda t: 1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride()))  # noqa: E731
+    ahead = (out.data_ptr() - logits.data_ptr()) // out.element_size()
+    if ahead >= reach(logits) or -ahead >= reach(out):
+        return False
+    if out.dim() == 2 and out.stride() == logits.stride() and out.shape[0] > 1:
+        n, pitch = out.shape[1], out.stride(0)
+        return not n <= ahead % pitch <= pitch - n
+    return True
+
+
 def _run(name, logits, actions, mask, temperature, top, saved=None, upstream=None, out=None, apart=False):
     """One library call.  saved: (entropy, row statistics) of an earlier forward pass, or None: forward values are made here.  upstream:
     the gradient's coefficients, or None: no gradient.  Returns (PolicyLogProbs or None, row statistics, gradient or None)."""
@@ -207,8 +223,8 @@ def policy_log_probs_grad(logits, actions=None, grad_log_prob=None, grad_entropy
             raise ValueError(f"out: expected {logits.dtype} {tuple(logits.shape)} on {dev}")
         if not (out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1 and out.stride(0) >= out.shape[1])):
             raise ValueError("out: rows must be dense and apart")
-        if out.data_ptr() == logits.data_ptr() and out.stride() != logits.stride():
-            raise ValueError("out: in place of the logits it must be the logits' own view")
+        if _overlap(out, logits):
+            raise ValueError("out overlaps the logits: it may be the logits' own view, or apart from them")
     values, _, grad = _run("mzs_policy_log_probs_train", logits, actions, mask, float(temperature), int(top), None,
                            coefficients, out)
     if out is not None:

@@ -412,6 +412,46 @@ def test_one_norm_for_two_optimizers_and_loss_scale():
     assert all(torch.equal(p, q) for p, q in zip(a + b, both))
 
 
+@pytest.mark.parametrize("dtype, count, bits", [(torch.float32, 70_000_003, 32), (torch.bfloat16, 140_000_003, 32), (torch.float32, 70_000_003, 8)])
+def test_long_lists_go_past_the_caches(dtype, count, bits):
+    """Arrays of more than 256 MiB; two steps, the second from states that the first wrote.  8 bits: against the same step in two halves,
+    each of them short enough to stay in the caches, and the first half (its dither counts from 0 as well) equal bit by bit."""
+    from muzero_amd.optim import AdamW, grad_norm
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randn(count, generator=g, device="cuda").to(dtype)
+    g1, g2 = (torch.randn(count, generator=g, device="cuda").mul_(0.01).to(dtype) for _ in range(2))
+    norm = grad_norm([g1, w])
+    want = float(torch.sqrt(sum((t.double() ** 2).sum() for t in (g1, w))))
+    assert abs(float(norm) - want) <= 4 * U * want
+    old = w.clone()
+    opt = AdamW([w], lr=0.01, weight_decay=0.1, state_bits=bits, seed=3)
+    opt.step([g1]), opt.step([g2])
+    if bits == 8:
+        half = 1 << 20
+        part = old[:half].clone()
+        other = AdamW([part], lr=0.01, weight_decay=0.1, state_bits=8, seed=3)
+        other.step([g1[:half].contiguous()]), other.step([g2[:half].contiguous()])
+        assert torch.equal(part, w[:half])
+        for k, v in other.state_tensors().items():
+            assert torch.equal(v.view(torch.uint8), opt.state_tensors()[k][:v.numel()].view(torch.uint8))
+        assert not torch.equal(w[-1000:], old[-1000:])
+        return
+    m = v = 0
+    x = old.double()
+    del old
+    for t, gr in ((1, g1.double()), (2, g2.double())):
+        m, v = 0.9 * m + 0.1 * gr, 0.999 * v + 0.001 * gr * gr
+        before = x
+        x = x * (1 - 0.001) - 0.01 / (1 - 0.9 ** t) * m / ((v / (1 - 0.999 ** t)).sqrt() + 1e-8)
+        if dtype is not torch.float32:      # the first step's weight may round the other way where it lies next to a border
+            rounded = x.to(dtype).double()
+            x = rounded
+    # each step's fp32 rounding: under 60 u lr and 2 u |w|; 2-byte weights round after each step, so the first one may differ by a step of theirs
+    eps = torch.finfo(dtype).eps
+    tol = 2 * (60 * U * 0.01 + 3 * U * x.abs()) + (2 * eps * torch.maximum(x.abs(), before.abs()) if dtype is not torch.float32 else 0.0)
+    assert bool(((w.double() - x).abs() <= tol).all())
+
+
 def test_saved_tensors_notice_the_step():
     from muzero_amd.optim import AdamW
     w = torch.ones(4, device="cuda", requires_grad=True)

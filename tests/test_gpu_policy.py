@@ -80,6 +80,7 @@ def exact_grad(e, actions, g_a, g_h, g_z, temperature, dtype):
         if 0 <= a[r] < n and e["ok"][r, a[r]]:
             g[r, a[r]] += g_a[r]
             tol[r, a[r]] += 4 * U * abs(g_a[r])
+    g[~e["ok"]] = 0.0       # forbidden actions' elements, also in a row that a NaN or an infinity poisons
     g, tol = g / temperature, tol / temperature
     smallest = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}[dtype]
     tol += (np.abs(g) + tol) * torch.finfo(dtype).eps / 2 + smallest
@@ -252,6 +253,61 @@ def test_gradient_in_place_and_in_a_wider_buffer(n, dtype):
     assert (wide[7:] == 7).all() and (wide[:, :5] == 7).all() and (wide[:, n + 5:] == 7).all()
     policy_log_probs_grad(x, a, g, g, mask=m, out=x)
     assert torch.equal(x, want)
+
+
+def test_gradient_beside_the_logits_and_overlapping_them():
+    from muzero_amd.policy import policy_log_probs_grad
+    x, a, _ = head(6, 40, torch.float32, 0)
+    g = torch.ones(6, device="cuda")
+    _, want = policy_log_probs_grad(x, a, g)
+    buffer = torch.zeros(12, 100, device="cuda")
+    for at, to in ((buffer[:6, :40], buffer[:6, 40:80]), (buffer[:6, 60:], buffer[:6, :40]), (buffer[:6, :40], buffer[6:, 3:43])):
+        at.copy_(x)
+        _, got = policy_log_probs_grad(at, a, g, out=to)
+        assert torch.equal(got, want) and torch.equal(at, x)
+    for at, to in ((buffer[:6, :40], buffer[:6, 39:79]), (buffer[:6, 60:], buffer[:6, 30:70]), (buffer[:6, :40], buffer[1:7, :40]),
+                   (buffer[:6, 60:], buffer[1:7, 59:99]), (buffer.view(-1)[:240].view(6, 40), buffer[:6, :40])):
+        with pytest.raises(ValueError):
+            policy_log_probs_grad(at, a, g, out=to)
+
+
+def test_saved_outputs_and_inputs_notice_a_change():
+    from muzero_amd.policy import policy_log_probs
+    x, a, m = head(6, 300, torch.float32, 0)
+    leaf = x.clone().requires_grad_()
+    for change in (lambda out: out.entropy.mul_(2), lambda out: a.zero_(), lambda out: m.fill_(True)):
+        out = policy_log_probs(leaf, a, mask=m)
+        loss = (out.log_prob + out.log_z).sum()
+        with torch.no_grad():
+            change(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            loss.backward()
+
+
+@pytest.mark.parametrize("R, n", [(256, 1025), (300, 2049), (257, 8193), (256, 20000), (260, 30011)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_wide_rows(R, n, dtype):
+    """Enough rows that a row is one block's, with and without alternatives; some rows of every kind among them."""
+    x, a, m = head(R, n, dtype, n)
+    m[3] = False
+    m[4] = False
+    m[4, n - 1] = True
+    x[5] = -math.inf
+    x[6] = torch.finfo(dtype).max
+    x[7] = torch.finfo(dtype).min
+    x[8, n // 2] = math.nan
+    x[9, 0] = math.inf
+    m[10, : n // 2], x[10, : n // 2] = False, math.nan
+    x[11] = 0.0
+    a[12] = -1
+    check(x, a, m, 0.5, top=7)
+    check(x[11:], a[11:], None, top=32)
+
+
+@pytest.mark.parametrize("R, n, dtype", [(4100, 2501, torch.bfloat16), (1500, 7001, torch.float32), (4096, 4096, torch.float16)])
+def test_gradients_of_long_lists(R, n, dtype):
+    x, a, m = head(R, n, dtype, R)
+    check(x, a, m, 1.3)
 
 
 def test_large_logits_keep_their_gradient():
