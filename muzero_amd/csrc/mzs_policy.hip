@@ -202,15 +202,38 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 constexpr int kBlock = 256;
 constexpr float kInf = __builtin_inff();
 
+/* a value of another lane, word by word */
+template <int kControl, typename V>
+__device__ __forceinline__ V from_lane(V v) {
+    uint32_t w[sizeof(V) / 4];
+    __builtin_memcpy(w, &v, sizeof(V));
+    _Pragma("unroll") for (uint32_t& x : w) x = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kControl, 0xf, 0xf, true);
+    __builtin_memcpy(&v, w, sizeof(V));
+    return v;
+}
+/* the values of lanes i and i ^ 16 (i ^ 32 with kRows = 2), in the same order for both */
+template <int kRows, typename V>
+__device__ __forceinline__ void both_lanes(V v, V& low, V& high) {
+    uint32_t w[sizeof(V) / 4], l[sizeof(V) / 4], h[sizeof(V) / 4];
+    __builtin_memcpy(w, &v, sizeof(V));
+    _Pragma("unroll") for (size_t i = 0; i < sizeof(V) / 4; ++i) {
+        const auto two = kRows == 1 ? __builtin_amdgcn_permlane16_swap(w[i], w[i], false, false)
+                                    : __builtin_amdgcn_permlane32_swap(w[i], w[i], false, false);
+        l[i] = two[0], h[i] = two[1];
+    }
+    __builtin_memcpy(&low, l, sizeof(V));
+    __builtin_memcpy(&high, h, sizeof(V));
+}
 /* Butterfly over G consecutive lanes: every lane gets the same bits (at each step both partners combine the same two values). */
-template <int G, typename F>
-__device__ __forceinline__ float lanes_reduce(float v, F op) {
-    if (G > 1) v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true)));   /* lane ^ 1 */
-    if (G > 2) v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true)));   /* lane ^ 2 */
-    if (G > 4) v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xf, 0xf, true)));  /* the other four of eight */
-    if (G > 8) v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xf, 0xf, true)));  /* the other eight of 16 */
-    if (G > 16) v = op(v, __shfl_xor(v, 16, 64));
-    if (G > 32) v = op(v, __shfl_xor(v, 32, 64));
+template <int G, typename V, typename F>
+__device__ __forceinline__ V lanes_reduce(V v, F op) {
+    if (G > 1) v = op(v, from_lane<0xB1>(v));  /* lane ^ 1 */
+    if (G > 2) v = op(v, from_lane<0x4E>(v));  /* lane ^ 2 */
+    if (G > 4) v = op(v, from_lane<0x141>(v)); /* the other four of eight */
+    if (G > 8) v = op(v, from_lane<0x140>(v)); /* the other eight of 16 */
+    V low, high;
+    if (G > 16) both_lanes<1>(v, low, high), v = op(low, high);
+    if (G > 32) both_lanes<2>(v, low, high), v = op(low, high);
     return v;
 }
 template <int G>
@@ -221,6 +244,55 @@ template <int G>
 __device__ __forceinline__ float lanes_sum(float v) {
     return lanes_reduce<G>(v, [](float a, float b) { return a + b; });
 }
+
+/* rank_key of a row of at most kRankMost logits in a register that one instruction compares: what the type's ranks differ in, then the inverted index.  next:
+ * the largest key below `last` in the team.  Fp32 (32 + 11 bits): as the mantissa of doubles, whose maximum is one instruction; 2-byte types
+ * (16 or 19 + 11 bits): key - last wraps for the keys below `last` and is largest for the nearest of them, so a maximum of differences finds it. */
+constexpr uint32_t kRankMost = MZS_POLICY_NARROW;
+template <typename T>
+struct Rank {
+    typedef uint32_t Key;
+    static constexpr uint32_t kDrop = sizeof(T) == 2 && Kind<T>::kNone == 0xff80u ? 16 : 13; /* low bits of the rank that say nothing */
+    static __device__ __forceinline__ Key first() { return 0x80000000u; }
+    static __device__ __forceinline__ Key make(float x, uint32_t i) {
+        return x == -kInf ? 0u : ((uint32_t)(rank_key(x, 0) >> 32) >> kDrop) * kRankMost + (kRankMost - 1 - i);
+    }
+    static __device__ __forceinline__ uint64_t whole(Key k) {
+        const uint32_t rank = k / kRankMost << kDrop;
+        return k == 0 ? 0 : (uint64_t)(rank | (rank & 0x80000000u ? 0u : (1u << kDrop) - 1u)) << 32 | (0xffffffffu - (kRankMost - 1 - k % kRankMost));
+    }
+    template <int G, int E>
+    static __device__ __forceinline__ Key next(const Key* key, Key last) {
+        Key best = 0u - last; /* nothing: key 0 */
+        _Pragma("unroll") for (int j = 0; j < E; ++j) best = max(best, key[j] - last);
+        best = lanes_reduce<G>(best, [](Key a, Key b) { return max(a, b); });
+        return last == 0 ? 0 : best + last;
+    }
+};
+template <>
+struct Rank<float> {
+    typedef double Key;
+    static __device__ __forceinline__ Key first() { return __longlong_as_double(0x7ff0000000000000ll); }
+    static __device__ __forceinline__ Key make(float x, uint32_t i) {
+        const uint64_t k = (uint64_t)(uint32_t)(rank_key(x, 0) >> 32) * kRankMost + (kRankMost - 1 - i);
+        return x == -kInf ? 0.0 : __longlong_as_double((long long)(k | 0x4000000000000000ull));
+    }
+    static __device__ __forceinline__ uint64_t whole(Key key) {
+        const uint64_t k = (uint64_t)__double_as_longlong(key) & 0x000fffffffffffffull;
+        return key == 0.0 ? 0 : k / kRankMost << 32 | (0xffffffffu - (kRankMost - 1 - (uint32_t)(k % kRankMost)));
+    }
+    static __device__ __forceinline__ Key larger(Key a, Key b) { /* neither is ever NaN: fmax would make sure of it first */
+        Key v;
+        asm("v_max_f64 %0, %1, %2" : "=v"(v) : "v"(a), "v"(b));
+        return v;
+    }
+    template <int G, int E>
+    static __device__ __forceinline__ Key next(const Key* key, Key last) {
+        Key best = 0.0;
+        _Pragma("unroll") for (int j = 0; j < E; ++j) best = larger(best, key[j] < last ? key[j] : 0.0);
+        return lanes_reduce<G>(best, larger);
+    }
+};
 
 /* c * big overflows, or its products lose the differences: such rows (the type's lowest values as a mask, all of them; 1e30 and
  * more) take their exponents as c (l_i - big) */
@@ -259,9 +331,13 @@ template <typename T>
 __device__ __forceinline__ float action_logit(const Row& p, const T* l, const uint8_t* mask, int64_t a) {
     return a < 0 || a >= p.n ? 0.0f : mask && !mask[a] ? -kInf : Kind<T>::load(l + a);
 }
+__device__ __forceinline__ int32_t top_action(uint64_t key) { return key ? (int32_t)(0xffffffffu - (uint32_t)key) : -1; }
+__device__ __forceinline__ float top_log_prob(const Row& p, uint64_t key, const Sum& v, const Values& o) {
+    return key ? p.scale * (key_value(key) - v.big) - o.log_total : -kInf;
+}
 __device__ __forceinline__ void write_top(const Row& p, int64_t r, int k, uint64_t key, const Sum& v, const Values& o) {
-    p.top_action[r * p.top + k] = key ? (int32_t)(0xffffffffu - (uint32_t)key) : -1;
-    p.top_log_prob[r * p.top + k] = key ? p.scale * (key_value(key) - v.big) - o.log_total : -kInf;
+    p.top_action[r * p.top + k] = top_action(key);
+    p.top_log_prob[r * p.top + k] = top_log_prob(p, key, v, o);
 }
 
 /* What the gradient of a row needs: grad_i = 2^(c l_i - m) (base + slope (c l_i - m)), + at_action where i is the action. */
@@ -293,78 +369,74 @@ __device__ __forceinline__ bool is_plain(const Row& p, const Slope& q) {
     return !q.empty && !is_huge(p, q.big) && fabsf(q.base) < kInf && fabsf(q.slope) < kInf;
 }
 
+/* Alternatives of a row whose team holds all its keys: the next one below the last, `top` times; the team's lanes write one each. */
+template <typename T, int kTeam, int E>
+__device__ __forceinline__ void write_best(const Row& p, int64_t r, int lane, const typename Rank<T>::Key* key, const Sum& v, const Values& o) {
+    typename Rank<T>::Key last = Rank<T>::first(), mine = last;
+    int k = 0;
+    if (kTeam == 1) { /* four to a store: 2M rows of 8 with all 8 of them 66 us, one at a time 98 */
+        for (; k + 4 <= p.top; k += 4) {
+            w4_any at, lp;
+            _Pragma("unroll") for (int i = 0; i < 4; ++i) {
+                last = Rank<T>::template next<1, E>(key, last);
+                const uint64_t whole = Rank<T>::whole(last);
+                at[i] = (uint32_t)top_action(whole), lp[i] = __float_as_uint(top_log_prob(p, whole, v, o));
+            }
+            *reinterpret_cast<w4_any*>(p.top_action + r * p.top + k) = at;
+            *reinterpret_cast<w4_any*>(p.top_log_prob + r * p.top + k) = lp;
+        }
+    }
+    for (; k < p.top; ++k) {
+        last = Rank<T>::template next<kTeam, E>(key, last);
+        const int turn = k % kTeam;
+        if (turn == lane) mine = last;
+        if ((turn == kTeam - 1 || k + 1 == p.top) && lane <= turn) write_top(p, r, k - turn + lane, Rank<T>::whole(mine), v, o);
+    }
+}
+
 /* ------------------------------------------------------------------ narrow rows
- * G lanes hold a row of up to G * E logits in registers, 64 / G rows to a wave: one read, one write, no shared memory.  The choice of
- * G and E by n is in launch_lanes. */
-template <typename T, int G, int E, bool kForward, bool kGrad, bool kTop>
+ * Up to 8 logits: a lane a row, in registers; one read, one write, nothing shared. */
+template <typename T, int E, bool kForward, bool kGrad, bool kTop>
 __global__ void __launch_bounds__(kBlock) k_policy_lanes(const Row p) {
-    constexpr int kRows = kBlock / G;
-    const int g = threadIdx.x % G;
     const int n = (int)p.n;
-    for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < p.rows; r0 += (int64_t)gridDim.x * kRows) {
-        const int64_t r_mine = r0 + threadIdx.x / G;
-        const bool live = r_mine < p.rows;
-        const int64_t r = live ? r_mine : p.rows - 1; /* lanes without a row shadow the last one: every lane takes part in the butterflies */
+    for (int64_t r = (int64_t)blockIdx.x * kBlock + threadIdx.x; r < p.rows; r += (int64_t)gridDim.x * kBlock) {
         const T* l = static_cast<const T*>(p.logits) + r * p.logits_stride;
         const uint8_t* mask = p.mask ? p.mask + r * p.mask_stride : nullptr;
         const int64_t a = row_action(p, r);
         float x[E];
-        _Pragma("unroll") for (int j = 0; j < E; ++j) {
-            const int i = g + j * G;
-            x[j] = i < n ? Kind<T>::load(l + i) : -kInf;
-        }
+        _Pragma("unroll") for (int i = 0; i < E; ++i) x[i] = i < n ? Kind<T>::load(l + i) : -kInf;
         if (mask) {
-            _Pragma("unroll") for (int j = 0; j < E; ++j) {
-                const int i = g + j * G;
-                if (i < n && !mask[i]) x[j] = -kInf;
-            }
+            _Pragma("unroll") for (int i = 0; i < E; ++i) if (i < n && !mask[i]) x[i] = -kInf;
         }
         const float la = kForward ? action_logit<T>(p, l, mask, a) : 0.0f;
         Sum v{-kInf, 0.0f, 0.0f};
-        _Pragma("unroll") for (int j = 0; j < E; ++j) v.big = fmaxf(v.big, x[j]);
-        v.big = lanes_max<G>(v.big);
+        _Pragma("unroll") for (int i = 0; i < E; ++i) v.big = fmaxf(v.big, x[i]);
         if (v.big > -kInf) {
-            _Pragma("unroll") for (int j = 0; j < E; ++j) {
-                const float d = exponent_of(p, x[j], v.big), e = power_of(d, x[j]);
+            _Pragma("unroll") for (int i = 0; i < E; ++i) {
+                const float d = exponent_of(p, x[i], v.big), e = power_of(d, x[i]);
                 v.s += e, v.t = fmaf(e, d, v.t);
             }
         } else { /* nothing allowed, or nothing but NaN */
-            _Pragma("unroll") for (int j = 0; j < E; ++j) if (x[j] != x[j]) v.s = x[j];
+            _Pragma("unroll") for (int i = 0; i < E; ++i) if (x[i] != x[i]) v.s = x[i];
         }
-        v.s = lanes_sum<G>(v.s), v.t = lanes_sum<G>(v.t);
         if (v.big == kInf) v.s = __builtin_nanf("");
         const Values o = row_values(p, v);
-        if (kForward && live && g == 0) write_row(p, r, v, o, la, a);
-        if (kTop) {
-            uint32_t key[E];
-            _Pragma("unroll") for (int j = 0; j < E; ++j)
-                key[j] = x[j] == -kInf ? 0u : (uint32_t)(rank_key(x[j], 0) >> 32);
-            uint64_t last = ~0ull;
-            for (int k = 0; k < p.top; ++k) {
-                uint64_t best = 0;
-                _Pragma("unroll") for (int j = 0; j < E; ++j) {
-                    const uint64_t c = key[j] ? ((uint64_t)key[j] << 32) | (0xffffffffu - (uint32_t)(g + j * G)) : 0;
-                    if (c < last && c > best) best = c;
-                }
-                _Pragma("unroll") for (int off = 1; off < G; off <<= 1) {
-                    const uint64_t other = __shfl_xor((unsigned long long)best, off, 64);
-                    best = other > best ? other : best;
-                }
-                last = best;
-                if (live && g == 0) write_top(p, r, k, last, v, o);
-            }
+        if (kForward) write_row(p, r, v, o, la, a);
+        if constexpr (kTop) {
+            typename Rank<T>::Key key[E];
+            _Pragma("unroll") for (int i = 0; i < E; ++i) key[i] = Rank<T>::make(x[i], (uint32_t)i);
+            write_best<T, 1, E>(p, r, 0, key, v, o);
         }
         if (kGrad) {
             const Slope q = row_slope(p, r, a, v, o.entropy, o.log2_s);
             T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
-            _Pragma("unroll") for (int j = 0; j < E; ++j) {
-                const int i = g + j * G;
+            _Pragma("unroll") for (int i = 0; i < E; ++i) {
                 float y = 0.0f;
-                if (!q.empty && x[j] != -kInf) {
-                    y = slope_at(p, q, x[j]);
+                if (!q.empty && x[i] != -kInf) {
+                    y = slope_at(p, q, x[i]);
                     if (i == a) y += q.at_action;
                 }
-                if (live && i < n) Kind<T>::store(out + i, y);
+                if (i < n) Kind<T>::store(out + i, y);
             }
         }
     }
@@ -809,7 +881,7 @@ __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks
  * block a row: blocks that start when others end keep loads, sums and stores of different rows in flight, where blocks that walk the rows
  * in step (two a CU, loading the next row into the registers just stored) took 292 us instead of 269 for 4096 x 81920 bf16.
  * Without alternatives: their search would hold its registers on top of the row's. */
-template <typename T, int kTeam, int V, bool kGrad>
+template <typename T, int kTeam, int V, bool kGrad, bool kTop = false>
 __global__ void __launch_bounds__(kTeam <= 64 ? kBlock : kTeam, kTeam <= 64 ? 1 : 4) k_policy_row(const Row p) {
     constexpr int kPer = Kind<T>::kPer;
     constexpr uint32_t kStride = kTeam * kPer;
@@ -845,6 +917,13 @@ __global__ void __launch_bounds__(kTeam <= 64 ? kBlock : kTeam, kTeam <= 64 ? 1 
     }
     const Values o = row_values(p, v);
     if (lane == 0 && p.values) write_row(p, r, v, o, la, a);
+    if constexpr (kTop) {
+        typename Rank<T>::Key key[V * kPer];
+        _Pragma("unroll") for (int j = 0; j < V; ++j)
+            _Pragma("unroll") for (int i = 0; i < kPer; ++i)
+                key[j * kPer + i] = Rank<T>::make(Kind<T>::get(x[j], i), lane * kPer + j * kStride + i);
+        write_best<T, kTeam, V * kPer>(p, r, (int)lane, key, v, o);
+    }
     if constexpr (kGrad) {
         const Slope q = row_slope(p, r, a, v, o.entropy, o.log2_s);
         T* out = static_cast<T*>(p.grad_logits) + r * p.grad_stride;
@@ -904,7 +983,6 @@ Row pack(const mzs_policy_args& a) {
     return p;
 }
 
-constexpr int64_t kLanesMost = MZS_POLICY_NARROW; /* widest row of k_policy_lanes */
 /* widest row whose gradient sums the row again in registers rather than read its statistics back */
 constexpr int64_t kRegainMost = 2048;
 
@@ -929,18 +1007,10 @@ Cut cut_row(int64_t rows, int64_t n, int per) {
 
 template <typename T, bool kForward, bool kGrad, bool kTop>
 void launch_lanes(const Row& p, hipStream_t st) {
-    const auto go = [&](auto kernel, int per_block) {
-        const int64_t blocks = (p.rows + per_block - 1) / per_block;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(kBlock), 0, st, p);
-    };
-    if (p.n <= 4) go(k_policy_lanes<T, 1, 4, kForward, kGrad, kTop>, 256);
-    else if (p.n <= 8) go(k_policy_lanes<T, 1, 8, kForward, kGrad, kTop>, 256);
-    else if constexpr (kTop) {
-        if (p.n <= 16) go(k_policy_lanes<T, 4, 4, kForward, kGrad, kTop>, 64);
-        else if (p.n <= 64) go(k_policy_lanes<T, 16, 4, kForward, kGrad, kTop>, 16);
-        else if (p.n <= 256) go(k_policy_lanes<T, 16, 16, kForward, kGrad, kTop>, 16);
-        else go(k_policy_lanes<T, 64, 16, kForward, kGrad, kTop>, 4);
-    }
+    const int64_t blocks = (p.rows + kBlock - 1) / kBlock;
+    const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
+    if (p.n <= 4) hipLaunchKernelGGL((k_policy_lanes<T, 4, kForward, kGrad, kTop>), grid, dim3(kBlock), 0, st, p);
+    else hipLaunchKernelGGL((k_policy_lanes<T, 8, kForward, kGrad, kTop>), grid, dim3(kBlock), 0, st, p);
 }
 
 template <typename T>
@@ -998,6 +1068,40 @@ void launch_wave_row(const Row& p, hipStream_t st) {
     else if (all <= 768) go(k_policy_row<T, 64, 12, kGrad>, 64);
     else go(k_policy_row<T, 64, 16, kGrad>, 64);
 }
+/* With alternatives, up to kRankMost logits: few lanes a row, as each choice costs its team's butterfly and then little for a row of
+ * 12 to 24 logits a lane - unless the rows are so few that their lanes do not fill the card, where more of them end sooner. */
+template <typename T>
+void launch_wave_top(const Row& p, hipStream_t st) {
+    constexpr int V = sizeof(T) == 4 ? 4 : 2, W = 3; /* fp32: 3 or 4 vectors a lane; 2-byte types: 2 or 3 */
+    constexpr int kSmall = V < W ? V : W, kLarge = V < W ? W : V;
+    const int64_t all = (p.n + Kind<T>::kPer - 1) / Kind<T>::kPer;
+    const auto go = [&](auto kernel, int team) {
+        const int64_t per_block = kBlock / team;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((p.rows + per_block - 1) / per_block)), dim3(kBlock), 0, st, p);
+    };
+    if (p.rows * all <= 64 * 2048 && all <= 64) {
+        if (all <= 4) go(k_policy_row<T, 4, 1, false, true>, 4);
+        else if (all <= 8) go(k_policy_row<T, 8, 1, false, true>, 8);
+        else if (all <= 16) go(k_policy_row<T, 16, 1, false, true>, 16);
+        else if (all <= 32) go(k_policy_row<T, 32, 1, false, true>, 32);
+        else go(k_policy_row<T, 64, 1, false, true>, 64);
+    } else if (all <= kSmall) go(k_policy_row<T, 1, kSmall, false, true>, 1);
+    else if (all <= kLarge) go(k_policy_row<T, 1, kLarge, false, true>, 1);
+    else if (all <= 2 * kSmall) go(k_policy_row<T, 2, kSmall, false, true>, 2);
+    else if (all <= 2 * kLarge) go(k_policy_row<T, 2, kLarge, false, true>, 2);
+    else if (all <= 4 * kSmall) go(k_policy_row<T, 4, kSmall, false, true>, 4);
+    else if (all <= 4 * kLarge) go(k_policy_row<T, 4, kLarge, false, true>, 4);
+    else if (all <= 8 * kSmall) go(k_policy_row<T, 8, kSmall, false, true>, 8);
+    else if (all <= 8 * kLarge) go(k_policy_row<T, 8, kLarge, false, true>, 8);
+    else if (all <= 16 * kSmall) go(k_policy_row<T, 16, kSmall, false, true>, 16);
+    else if (all <= 16 * kLarge) go(k_policy_row<T, 16, kLarge, false, true>, 16);
+    else if (all <= 32 * kSmall) go(k_policy_row<T, 32, kSmall, false, true>, 32);
+    else if (all <= 32 * kLarge) go(k_policy_row<T, 32, kLarge, false, true>, 32);
+    else if (all <= 64 * kSmall) go(k_policy_row<T, 64, kSmall, false, true>, 64);
+    else if (all <= 64 * kLarge) go(k_policy_row<T, 64, kLarge, false, true>, 64);
+    else if (sizeof(T) == 4 && all <= 64 * 6) go(k_policy_row<T, 64, sizeof(T) == 4 ? 6 : 2 * V, false, true>, 64);
+    else go(k_policy_row<T, 64, 2 * V, false, true>, 64);
+}
 template <typename T>
 void launch_block_row(const Row& p, hipStream_t st) {
     const int64_t all = (p.n + (int64_t)kRowThreads * Kind<T>::kPer - 1) / ((int64_t)kRowThreads * Kind<T>::kPer);
@@ -1037,7 +1141,7 @@ Row rows_from(Row p, int64_t r, int64_t rows) {
  *   beyond                      chunks and their join; the gradient from the statistics     k_policy_chunk, k_policy_join, k_policy_slope */
 template <typename T>
 void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool forward, bool grad) {
-    const bool wave = fits_wave<T>(all.n) && all.n > 8, lanes = all.n <= kLanesMost;
+    const bool wave = fits_wave<T>(all.n) && all.n > 8, lanes = all.n <= 8;
     const int64_t slab = wave || lanes ? (int64_t)1 << 24 : kSlab;
     for (int64_t r = 0; r < all.rows; r += slab) {
         const Row p = rows_from<T>(all, r, all.rows - r < slab ? all.rows - r : slab);
@@ -1056,6 +1160,7 @@ void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool for
         }
         if (forward) {
             if (wave && p.top == 0) launch_wave_row<T, false>(p, st);
+            else if (wave && p.n <= kRankMost) launch_wave_top<T>(p, st);
             else if (lanes && p.top > 0) launch_lanes<T, true, false, true>(p, st);
             else if (lanes) launch_lanes<T, true, false, false>(p, st);
             else launch_forward<T>(p, a, st);
@@ -1064,14 +1169,14 @@ void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool for
             Row g = p;
             g.values = 0;
             if (wave && p.n <= kRegainMost) launch_wave_row<T, true>(g, st);
-            else if (p.n <= 8) launch_lanes<T, false, true, false>(p, st);
+            else if (lanes) launch_lanes<T, false, true, false>(p, st);
             else launch_slope<T>(p, st);
         }
     }
 }
 
 size_t workspace_bytes(const mzs_policy_args& a, int per) {
-    if (a.rows == 0 || a.n_actions <= kLanesMost) return 0; /* MZS_POLICY_NARROW */
+    if (a.rows == 0 || a.n_actions <= MZS_POLICY_NARROW) return 0;
     const Cut c = cut_row(a.rows, a.n_actions, per);
     if (c.chunks == 1) return 0;
     return sizeof(float) * (size_t)a.rows * c.chunks * (3 + (a.top > 0 ? kStripsPerBlock : 0));

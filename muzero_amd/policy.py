@@ -180,15 +180,22 @@ class _LogProbs(torch.autograd.Function):
         return tuple(out)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_log_prob, g_entropy, g_log_z, *_):
-        if g_log_prob is None and g_entropy is None and g_log_z is None:
-            return None, None, None, None, None
-        logits, actions, mask, entropy, stats = ctx.saved_tensors
-        lead, device = logits.shape[:-1], logits.device
-        upstream = [_coefficient(g, "gradient", lead, device) for g in (g_log_prob, g_entropy, g_log_z)]
-        _, _, grad = _run("mzs_policy_log_probs_grad", logits, actions, mask, ctx.temperature, 0, (entropy, stats), upstream)
-        return grad, None, None, None, None
+    def backward(ctx, *grads):
+        # once_differentiable's bookkeeping costs as much as the launch: only where a graph of the gradient is asked for
+        return (_slope_once if torch.is_grad_enabled() else _slope)(ctx, *grads)
+
+
+def _slope(ctx, g_log_prob, g_entropy, g_log_z, *_):
+    if g_log_prob is None and g_entropy is None and g_log_z is None:
+        return None, None, None, None, None
+    logits, actions, mask, entropy, stats = ctx.saved_tensors
+    lead, device = logits.shape[:-1], logits.device
+    upstream = [g if g is None else _coefficient(g, "gradient", lead, device) for g in (g_log_prob, g_entropy, g_log_z)]
+    _, _, grad = _run("mzs_policy_log_probs_grad", logits, actions, mask, ctx.temperature, 0, (entropy, stats), upstream)
+    return grad, None, None, None, None
+
+
+_slope_once = torch.autograd.function.once_differentiable(_slope)
 
 
 def policy_log_probs(logits, actions=None, mask=None, temperature=1.0, top=0):
