@@ -537,7 +537,7 @@ __device__ Sum sum_slowly(const Row& p, const T* l, const uint8_t* mask, uint32_
 constexpr int kStrips = 512; /* strips that can hold alternatives              */
 constexpr int kKeys = 1024;  /* logits that can be alternatives                */
 constexpr int kGroups = kBlock / 4; /* four threads' strips: enough groups for MZS_POLICY_MAX_TOP of them */
-static_assert(kBlock / 64 <= kGroups && MZS_POLICY_MAX_TOP <= kGroups, "tau is one of the groups' maxima");
+static_assert(kGroups == 64 && MZS_POLICY_MAX_TOP <= kGroups, "tau is one of the groups' maxima, a lane's each");
 struct TopScratch {
     uint64_t keys[kKeys];
     uint32_t strips[kStrips];
@@ -551,7 +551,6 @@ __device__ __forceinline__ uint32_t rank_value(float x) { return x == -kInf ? 0u
 
 constexpr int kStripLanes = 4;                     /* neighbouring threads whose vectors make a strip */
 constexpr int kStripsPerBlock = kBlock / kStripLanes;
-static_assert(kStripsPerBlock == kBlock / 4 && kStripLanes == 4, "held_strip gives a lone chunk its own threads");
 constexpr int kHold = 16; /* strips of a row that a thread holds in registers */
 /* strip in held[h] of this thread; >= n_strips: none.  Few strips are spread over the block, so that every group has one. */
 __device__ __forceinline__ int held_strip(int h, int n_strips) {
@@ -560,42 +559,47 @@ __device__ __forceinline__ int held_strip(int h, int n_strips) {
     return at % spread ? n_strips : at / spread;
 }
 
-/* Alternatives from strips.  A strip is the vectors that kStripLanes threads took of one chunk; its largest logit is known.  Each four of
- * the block's threads take the largest over their share of the strips; tau, the top-th largest of those 64, is reached by at least `top`
- * logits, so
+/* Alternatives from strips.  A strip is the vectors that kLanes neighbouring threads took of one chunk; its largest logit is known.  Each
+ * four of the block's threads take the largest over their share of the strips; tau, the top-th largest of those 64, is reached by at least
+ * `top` logits, so
  *   1. strips whose maximum reaches tau are read again and their logits that reach it collected — hardly more than `top` of them, as
  *      the best ones seldom share a group (top 20: 24 on the average, top 32: 44);
  *   2. a collected logit's rank is the number of collected ones before it.
- * Both need little more than the strips' maxima (1 / 64 of the row or less), whatever the logits — unless many are alike: where they do not
+ * Both need little more than the strips' maxima, whatever the logits — unless many are alike: where they do not
  * fit the lists, only those above tau are collected, and the ones equal to tau are taken from the row's start on.  A row where
- * even that is too much (or with NaN) is searched `top` times.  Every choice is by value and index: the lists' order does not matter. */
-template <typename T, typename Maximum>
+ * even that is too much (or with NaN) is searched `top` times.  Every choice is by value and index: the lists' order does not matter.
+ * A row that one block has whole knows its threads' own maxima (kLanes 1: a 256th of the row for each alternative is read again); strips
+ * that travel through memory to the join are four threads' each (a 64th of what the block took). */
+template <typename T, int kLanes, int kHeld, typename Maximum>
 __device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* mask, const Sum& v, const Values& o, const float* held, Maximum maximum,
                            int n_strips, int chunk_vecs, uint32_t chunk_len, TopScratch& sh) {
     constexpr int kPer = Kind<T>::kPer;
+    constexpr uint32_t kPerBlock = kBlock / kLanes;
     const int tid = threadIdx.x;
     const uint32_t want = (uint32_t)p.top, n = (uint32_t)p.n;
     const bool plain = v.s == v.s;
     uint32_t mine = 0;
-    _Pragma("unroll") for (int h = 0; h < kHold; ++h) mine = max(mine, rank_value(held[h]));
-    for (int i = tid + kHold * kBlock; i < n_strips; i += kBlock) mine = max(mine, rank_value(maximum(i)));
-    uint32_t group = max(mine, (uint32_t)__builtin_amdgcn_mov_dpp((int)mine, 0xB1, 0xf, 0xf, true));
-    group = max(group, (uint32_t)__builtin_amdgcn_mov_dpp((int)group, 0x4E, 0xf, 0xf, true));
+    _Pragma("unroll") for (int h = 0; h < kHeld; ++h) mine = max(mine, rank_value(held[h]));
+    for (int i = tid + kHeld * kBlock; i < n_strips; i += kBlock) mine = max(mine, rank_value(maximum(i)));
+    const uint32_t group = lanes_reduce<4>(mine, [](uint32_t a, uint32_t b) { return max(a, b); });
     if (tid % 4 == 0) sh.groups[tid / 4] = group;
-    if (tid == 0) sh.tau = 0xffffffffu;
+    if (tid == 0) sh.n_strips = 0, sh.n_keys = 0;
     __syncthreads();
-    uint32_t ahead = 0; /* groups with a larger one */
-    _Pragma("unroll") for (int i = 0; i < kGroups / 4; ++i) {
-        const w4 g = *reinterpret_cast<const w4*>(sh.groups + 4 * i);
-        _Pragma("unroll") for (int j = 0; j < 4; ++j) ahead += g[j] > group;
+    if (tid < kGroups) { /* a wave */
+        const uint32_t g = sh.groups[tid];
+        uint32_t ahead = 0; /* groups with a larger one */
+        _Pragma("unroll") for (int i = 0; i < kGroups; ++i) ahead += (uint32_t)__builtin_amdgcn_readlane((int)g, i) > g;
+        const uint32_t least = lanes_reduce<kGroups>(ahead < want ? g : 0xffffffffu, [](uint32_t a, uint32_t b) { return min(a, b); });
+        if (tid == 0) sh.tau = least; /* the smallest of those that fewer than `top` are ahead of */
     }
-    if (ahead < want) atomicMin(&sh.tau, group); /* the smallest of those that fewer than `top` are ahead of */
     bool done = false;
     for (int stage = 0; stage < 2 && plain && !done; ++stage) {
         __syncthreads();
         const uint32_t tau = sh.tau, least = stage ? tau + 1u : max(tau, 1u);
-        if (tid == 0) sh.n_strips = 0, sh.n_keys = 0;
-        __syncthreads();
+        if (stage) {
+            if (tid == 0) sh.n_strips = 0, sh.n_keys = 0;
+            __syncthreads();
+        }
         const auto look = [&](float largest, int i) {
             if (rank_value(largest) >= least) {
                 const uint32_t at = atomicAdd(&sh.n_strips, 1u);
@@ -603,16 +607,15 @@ __device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* m
             }
         };
         if (mine >= least) {
-            _Pragma("unroll") for (int h = 0; h < kHold; ++h) look(held[h], held_strip(h, n_strips));
-            for (int i = tid + kHold * kBlock; i < n_strips; i += kBlock) look(maximum(i), i);
+            _Pragma("unroll") for (int h = 0; h < kHeld; ++h) look(held[h], kLanes == 1 ? tid : held_strip(h, n_strips));
+            for (int i = tid + kHeld * kBlock; i < n_strips; i += kBlock) look(maximum(i), i);
         }
         __syncthreads();
-        const uint32_t found = sh.n_strips, each = (uint32_t)chunk_vecs * kStripLanes;
+        const uint32_t found = sh.n_strips, each = (uint32_t)chunk_vecs * kLanes;
         if (found <= kStrips) {
             for (uint32_t w = tid; w < found * each; w += kBlock) {
-                const uint32_t strip = sh.strips[w / each], lane = w % kStripLanes, j = w % each / kStripLanes;
-                const uint32_t i =
-                    skew_of(l) + strip / kStripsPerBlock * chunk_len + (j * kBlock + strip % kStripsPerBlock * kStripLanes + lane) * kPer;
+                const uint32_t strip = sh.strips[w / each], lane = w % kLanes, j = w % each / kLanes;
+                const uint32_t i = skew_of(l) + strip / kPerBlock * chunk_len + (j * kBlock + strip % kPerBlock * kLanes + lane) * kPer;
                 if (i >= n) continue;
                 const w4 x = load_vec<T>(l, mask, i, n);
                 _Pragma("unroll") for (int q = 0; q < kPer; ++q) {
@@ -725,25 +728,34 @@ __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks
         dress<T, kAhead>(mask, from + (uint32_t)g * kAhead * kStride, kStride, n, v);
         take_vecs<T, kAhead>(p, v, sum);
     };
+    const auto rest = [&](auto count) { /* what the groups leave, together */
+        constexpr int N = decltype(count)::value;
+        const uint32_t i = from + (uint32_t)groups * kAhead * kStride;
+        w4 z[N];
+        load_vecs<T, N>(l, mask, i, kStride, n, z);
+        take_vecs<T, N>(p, z, sum);
+    };
     load(0, x);
+    static_assert(kAhead == 4, "a case for each rest");
+    switch (chunk_vecs % kAhead) {
+        case 1: rest(std::integral_constant<int, 1>()); break;
+        case 2: rest(std::integral_constant<int, 2>()); break;
+        case 3: rest(std::integral_constant<int, 3>()); break;
+    }
     for (int g = 0; g < groups; g += 2) {
         load(g + 1, y);
         take(g, x);
         load(g + 2, x);
         if (g + 1 < groups) take(g + 1, y);
     }
-    for (int j = groups * kAhead; j < chunk_vecs; ++j) {
-        w4 z = load_vec<T>(l, mask, from + (uint32_t)j * kStride, n);
-        take_vecs<T, 1>(p, &z, sum);
-    }
     if (skew && from == skew) take_one(p, extra, sum);
-    const float strip = lanes_max<kStripLanes>(sum.big);
     Sum v = team_merge<kBlock>(p, running_end(p, sum), lds);
     if (is_huge(p, v.big) && fabsf(v.big) < kInf) {
         __syncthreads();
         v = team_merge<kBlock>(p, sum_slowly<T>(p, l, mask, from, kBlock * kPer, skew + (chunk + 1) * chunk_len, n, v.big, extra), lds);
     }
     if constexpr (kSplit) {
+        const float strip = lanes_max<kStripLanes>(sum.big);
         if (p.top > 0 && threadIdx.x % kStripLanes == 0)
             strips[(int64_t)blockIdx.x * kStripsPerBlock + threadIdx.x / kStripLanes] = strip;
         if (threadIdx.x == 0) {
@@ -755,10 +767,7 @@ __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks
         const Values o = row_values(p, v);
         if (threadIdx.x == 0) write_row(p, r, v, o, la, a);
         if (p.top > 0) {
-            float held[kHold];
-            _Pragma("unroll") for (int h = 0; h < kHold; ++h)
-                held[h] = held_strip(h, kStripsPerBlock) < kStripsPerBlock ? strip : -kInf; /* a strip's own threads hold it */
-            select_top<T>(p, r, l, mask, v, o, held, [](int) { return -kInf; }, kStripsPerBlock, chunk_vecs, chunk_len, top);
+            select_top<T, 1, 1>(p, r, l, mask, v, o, &sum.big, [](int) { return -kInf; }, kBlock, chunk_vecs, chunk_len, top);
         }
     }
 }
@@ -791,7 +800,7 @@ __global__ void __launch_bounds__(kBlock) k_policy_join(const Row p, int chunks,
     const Values o = row_values(p, v);
     if (threadIdx.x == 0) write_row(p, r, v, o, la, a);
     if (p.top > 0)
-        select_top<T>(p, r, l, mask, v, o, held, [&](int i) { return mine[i]; }, n_strips, chunk_vecs,
+        select_top<T, kStripLanes, kHold>(p, r, l, mask, v, o, held, [&](int i) { return mine[i]; }, n_strips, chunk_vecs,
                       (uint32_t)chunk_vecs * kBlock * Kind<T>::kPer, top);
 }
 
