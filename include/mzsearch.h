@@ -430,7 +430,7 @@ int mzs_replay_update_value(int32_t batch, int32_t num_unroll, double* const* ro
 #define MZS_DTYPE_HALF 2
 #define MZS_POLICY_MAX_TOP 32
 #define MZS_POLICY_NARROW 2048 /* rows of at most so many logits need no workspace, */
-#define MZS_POLICY_MANY 256    /* nor do calls of at least so many rows            */
+#define MZS_POLICY_MANY 128    /* nor do calls of at least so many rows            */
 
 typedef struct mzs_policy_args {
     int32_t device;             /* HIP device of every pointer below                                  */

@@ -50,7 +50,7 @@ class Config(C.Structure):
 
 
 DTYPE_FLOAT, DTYPE_BFLOAT, DTYPE_HALF = 0, 1, 2
-POLICY_MAX_TOP, POLICY_NARROW, POLICY_MANY = 32, 2048, 256
+POLICY_MAX_TOP, POLICY_NARROW, POLICY_MANY = 32, 2048, 128
 OPTIM_ALIGN, OPTIM_BLOCK, OPTIM_ENTRY_BYTES, OPTIM_CONTROL_BYTES = 64, 32, 32, 64
 
 

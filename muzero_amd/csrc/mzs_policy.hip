@@ -44,7 +44,7 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
-/* A logit type: kPer elements in 16 bytes.  get / set work on 16 bytes in registers, element j by a constant index. */
+/* A logit type: kPer elements in 16 bytes.  get: element j (a constant) of 16 bytes in registers. */
 template <typename T>
 struct Kind;
 template <>
@@ -54,7 +54,6 @@ struct Kind<float> {
     static __device__ __forceinline__ float load(const float* p) { return *p; }
     static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
     static __device__ __forceinline__ float get(const w4& v, int j) { return __uint_as_float(v[j]); }
-    static __device__ __forceinline__ void set(w4& v, int j, float x) { v[j] = __float_as_uint(x); }
     static __device__ __forceinline__ void keep(w4& v, const uint32_t* m) { /* a byte of m for each */
         _Pragma("unroll") for (int j = 0; j < 4; ++j) v[j] = (m[0] >> (8 * j)) & 0xffu ? v[j] : kNone;
     }
@@ -159,9 +158,11 @@ __device__ __forceinline__ w4 load_vec(const T* __restrict__ l, const uint8_t* _
     load_vecs<T, 1>(l, mask, i, 0, n, &x);
     return x;
 }
-template <typename T>
+template <typename T, bool kStream = false>
 __device__ __forceinline__ void store_vec(T* __restrict__ g, uint32_t i, const w4& v) {
-    *reinterpret_cast<w4_any*>(reinterpret_cast<char*>(g) + (uint32_t)(i * sizeof(T))) = v;
+    w4_any* to = reinterpret_cast<w4_any*>(reinterpret_cast<char*>(g) + (uint32_t)(i * sizeof(T)));
+    if constexpr (kStream) __builtin_nontemporal_store(v, to);
+    else *to = v;
 }
 
 /* Wide rows of 2-byte logits at an odd element: their vectors start at the row's second logit, so that every one is 4-byte aligned (a
@@ -395,7 +396,8 @@ __device__ __forceinline__ void write_best(const Row& p, int64_t r, int lane, co
 }
 
 /* ------------------------------------------------------------------ narrow rows
- * Up to 8 logits: a lane a row, in registers; one read, one write, nothing shared. */
+ * Up to 8 logits: a lane a row, in registers; one read, one write, nothing shared.  Bound by memory: 2M x 4 fp32 with the best action
+ * 22 us, 4.1 TB/s of what it reads and writes; 4096 rows 3.3 us, of which an empty launch is 2.5. */
 template <typename T, int E, bool kForward, bool kGrad, bool kTop>
 __global__ void __launch_bounds__(kBlock) k_policy_lanes(const Row p) {
     const int n = (int)p.n;
@@ -703,7 +705,11 @@ __device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* m
     }
 }
 
-/* kSplit: the chunk's part goes to parts[row][chunk] and its strips' maxima to strips[row][chunk][thread]; else the chunk is the row */
+/* Forward pass of a chunk: one read, running maximum and sums, four vectors a thread on their way while four are summed.  kSplit: the
+ * chunk's part goes to parts[row][chunk] and its strips' maxima to strips[row][chunk][strip]; else the chunk is the row.  Bound by the read
+ * and, beside it, by the arithmetic (an element's exponential and eight more operations take half the time of its read): 640 x 100000 bf16
+ * from memory 30 us, 4.2 TB/s, 39 with the five best alternatives, whose search every block ends with at once; two vectors in flight 30,
+ * six 33, at least six waves a SIMD (fewer registers) 33. */
 template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks, int chunk_vecs, float* __restrict__ parts,
                                                          float* __restrict__ strips) {
@@ -772,7 +778,8 @@ __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks
     }
 }
 
-/* joins the parts of each row's chunks (at most kBlock of them) */
+/* Joins the parts of each row's chunks (at most kBlock of them).  Bound by latency, one block's chain of loads and barriers: one row of 83521
+ * with 20 alternatives 8 us, behind 3.3 us of k_policy_chunk. */
 template <typename T>
 __global__ void __launch_bounds__(kBlock) k_policy_join(const Row p, int chunks, int chunk_vecs, const float* __restrict__ parts,
                                                         const float* __restrict__ strips) {
@@ -847,8 +854,9 @@ __device__ __forceinline__ void store_action(const Row& p, const Slope& q, float
 
 /* Gradient of chunks from the rows' stored statistics; kSlopeGroups groups of vectors a thread, each on its way while the one before it is
  * worked on, the first while the row's statistics come.  1280 x 59049 fp16: 48.8 us with four groups, 52.8 with two, 54.6 with
- * one, which few rows get for the sake of more blocks. */
-template <typename T, int kSlopeGroups>
+ * one, which few rows get for the sake of more blocks.  kStream: past the caches, for gradients that do not fit the 256 MiB last-level cache
+ * beside the logits, which the forward pass left there: forward and gradient of the same 1280 rows 96 -> 86 us. */
+template <typename T, int kSlopeGroups, bool kStream>
 __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks) {
     constexpr int kPer = Kind<T>::kPer;
     constexpr uint32_t kStride = kBlock * kPer, kLen = kSlopeGroups * kAhead * kStride;
@@ -876,7 +884,7 @@ __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks
         dress<T, kAhead>(mask, i, kStride, n, x[g & 1]);
         _Pragma("unroll") for (int u = 0; u < kAhead; ++u) {
             const uint32_t at = i + u * kStride;
-            if (at < whole) store_vec<T>(out, at, slope_vec<T>(p, q, x[g & 1][u]));
+            if (at < whole) store_vec<T, kStream>(out, at, slope_vec<T>(p, q, x[g & 1][u]));
         }
     }
     if (whole >= first && whole < end) slope_slowly<T, kBlock>(p, q, l, mask, out, whole, n, action);
@@ -889,7 +897,8 @@ __global__ void __launch_bounds__(kBlock) k_policy_slope(const Row p, int chunks
  * rows of up to 16 vectors a thread; a block of 512 threads wider ones, two blocks to a CU (at most 128 registers a thread), one
  * block a row: blocks that start when others end keep loads, sums and stores of different rows in flight, where blocks that walk the rows
  * in step (two a CU, loading the next row into the registers just stored) took 292 us instead of 269 for 4096 x 81920 bf16.
- * Without alternatives: their search would hold its registers on top of the row's. */
+ * kTop: alternatives too, from keys beside the row (Rank), so rows of at most kRankMost logits; 80000 x 1000 bf16 with the five best 84 us,
+ * 62 for 40000 x 1000 fp32, where a maximum of 64-bit keys through shared memory took 214 and 73. */
 template <typename T, int kTeam, int V, bool kGrad, bool kTop = false>
 __global__ void __launch_bounds__(kTeam <= 64 ? kBlock : kTeam, kTeam <= 64 ? 1 : 4) k_policy_row(const Row p) {
     constexpr int kPer = Kind<T>::kPer;
@@ -995,16 +1004,18 @@ Row pack(const mzs_policy_args& a) {
 /* widest row whose gradient sums the row again in registers rather than read its statistics back */
 constexpr int64_t kRegainMost = 2048;
 
-/* How a wide row is cut: `chunks` blocks a row, each thread `vecs` vectors.  Rows are cut where there are fewer of them than CUs: from
- * there on a block a row keeps up (us without / with the five best alternatives, 320 x 59049 bf16: 15 / 21 whole, 20 / 25 cut; 1280 x
- * 20000: 16 / 21 and 20 / 27; 640 x 100000 the same; 160 x 100000 fp32: 19 / 24 cut). */
+/* How a wide row is cut: `chunks` blocks a row, each thread `vecs` vectors.  Only few and long rows are: a block alone reads 12000 bf16 a us,
+ * and the join costs a launch and a second search (us whole / cut, without alternatives and with five, logits from memory: 8 x 100000 bf16
+ * - and 15 / 10, 64 of them 13 / 11 and 17 / 15, 100 13 / 13, 160 16 / 19 and 20 / 23; 8 x 50000 - and 10 / 10; 8 x 20000 - and 7.7 / 9.7, 64 5.5 / 6.9
+ * and 8.4 / 11; fp32 32 x 100000 19 / 18 with, one of 30000 8 / 9). */
 struct Cut {
     int chunks, vecs;
 };
+constexpr int64_t kCutLeast = 49152;
 Cut cut_row(int64_t rows, int64_t n, int per) {
     const int64_t all = (n + (int64_t)kBlock * per - 1) / ((int64_t)kBlock * per); /* vectors a thread would have of a whole row */
     int64_t chunks = 1;
-    if (rows < MZS_POLICY_MANY) chunks = (8192 + rows - 1) / rows;
+    if (rows < MZS_POLICY_MANY && n >= kCutLeast) chunks = (8192 + rows - 1) / rows;
     if (chunks > kBlock) chunks = kBlock;
     if (chunks > all) chunks = all;
     Cut c;
@@ -1039,10 +1050,12 @@ template <typename T>
 void launch_slope(const Row& p, hipStream_t st) {
     const int64_t group = (int64_t)kAhead * kBlock * Kind<T>::kPer, groups = (p.n + group - 1) / group;
     if (p.rows * groups < 4096) {
-        hipLaunchKernelGGL((k_policy_slope<T, 1>), dim3((unsigned)(p.rows * groups)), dim3(kBlock), 0, st, p, (int)groups);
+        hipLaunchKernelGGL((k_policy_slope<T, 1, false>), dim3((unsigned)(p.rows * groups)), dim3(kBlock), 0, st, p, (int)groups);
     } else {
         const int chunks = (int)((groups + 3) / 4);
-        hipLaunchKernelGGL((k_policy_slope<T, 4>), dim3((unsigned)(p.rows * chunks)), dim3(kBlock), 0, st, p, chunks);
+        const bool stream = 2 * p.rows * p.n * (int64_t)sizeof(T) > ((int64_t)256 << 20);
+        hipLaunchKernelGGL((stream ? k_policy_slope<T, 4, true> : k_policy_slope<T, 4, false>), dim3((unsigned)(p.rows * chunks)), dim3(kBlock), 0,
+                           st, p, chunks);
     }
 }
 
@@ -1144,8 +1157,7 @@ Row rows_from(Row p, int64_t r, int64_t rows) {
 }
 /* The ways, by the width of the row (and how a call needs it):
  *   up to 8 logits              a lane a row, a logit at a time                             k_policy_lanes
- *   up to 16 vectors a lane     a row in a team's registers, without alternatives           k_policy_row, teams up to a wave
- *   up to 1024                  alternatives                                                k_policy_lanes
+ *   up to 16 vectors a lane     a row in a team's registers; with alternatives up to 2048   k_policy_row, teams up to a wave
  *   up to 24 vectors a thread   forward and gradient of a row in a block's registers        k_policy_row, a block
  *   beyond                      chunks and their join; the gradient from the statistics     k_policy_chunk, k_policy_join, k_policy_slope */
 template <typename T>
