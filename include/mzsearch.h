@@ -422,8 +422,8 @@ int mzs_replay_update_value(int32_t batch, int32_t num_unroll, double* const* ro
  * A row that allows nothing (all masked or -inf): log_z = log_prob = -inf, entropy 0, gradient 0, no alternatives.
  * Action < 0: the row has none (log_prob 0, g_a not used).  Action >= n_actions: log_prob NaN.  Action forbidden:
  * log_prob -inf, and its own gradient element stays 0.  A NaN or +inf among the allowed logits makes the row's values and
- * gradient NaN (alternatives: NaN ranks first), forbidden actions' gradient is 0 there too; masked logits are never looked at.  Slots of alternatives beyond the allowed
- * actions hold index -1 and -inf.
+ * gradient NaN (alternatives: NaN ranks first; forbidden actions' gradient is 0 there too); masked logits are never
+ * looked at.  Slots of alternatives beyond the allowed actions hold index -1 and -inf.
  * Everything is computed in fp32; logits and gradient are fp32, bf16 or fp16. */
 #define MZS_DTYPE_FLOAT 0
 #define MZS_DTYPE_BFLOAT 1
@@ -490,7 +490,7 @@ int mzs_optim_table(int32_t device, int32_t n, const void* const* pointers, cons
 /* bytes of workspace for a norm over n_tiles tiles (zeroed once by nobody: its contents are written before they are read) */
 size_t mzs_grad_norm_workspace(int64_t n_tiles);
 
-/* norm_dev[0] = grad_scale * sqrt(sum of squares over every tensor of the table), summed in fp64 in a fixed order.
+/* norm_dev[0] = |grad_scale| sqrt(sum of squares over every tensor of the table), summed in fp64 in a fixed order.
  * dtype: MZS_DTYPE_* of all tensors. */
 int mzs_grad_norm(int32_t device, int32_t n, const void* table_dev, int64_t n_tiles, int32_t dtype, double grad_scale,
                   float* norm_dev, void* workspace, size_t workspace_bytes, void* stream);
