@@ -452,3 +452,70 @@ def test_many_short_rows():
     flat, one = math.log(n), math.log(n - 1 + math.exp(3.0))
     assert abs(out.log_z[0].item() - flat) < 1e-4 and abs(out.log_z[-1].item() - one) < 1e-4
     assert abs(out.log_prob[-1].item() - (3.0 - one)) < 1e-4
+
+
+@pytest.mark.parametrize("n", [9, 10, 12, 13, 16, 17, 24, 25, 32, 33, 48, 64, 65, 96, 127, 128, 192, 200, 256, 384, 500, 512, 700, 768, 1000,
+                               1024, 1025, 1300, 1536, 1537, 2000, 2047, 2048])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_alternatives_of_many_rows(n, dtype):
+    """Enough rows that few lanes hold each: 96 rows with ties, forbidden and infinite places over and over, the last ones cut off."""
+    R, top = 96, (1, 7, 32)[n % 3]
+    x, a, m = head(R, n, dtype, n)
+    x[:40] = (x[:40] * 2).round() / 2
+    x[40], x[41, n // 2:], m[42] = -math.inf, -math.inf, False
+    m[43:48] = True
+    x[44] = torch.finfo(dtype).min
+    x[45] = 0.0
+    e = exact(x, a, m, 0.5, top)
+    times = 131072 * 8 // (R * n) + 2
+    rows = R * times - 5
+    from muzero_amd.policy import policy_log_probs
+    o = policy_log_probs(x.repeat(times, 1)[:rows], a.repeat(times)[:rows], mask=m.repeat(times, 1)[:rows], temperature=0.5, top=top)
+    index = np.arange(rows) % R
+    assert np.array_equal(o.top_action.cpu().numpy(), e["top_at"][index])
+    t = e["tol_z"][:, None] + 3 * U * np.where(np.isfinite(e["top"]), np.abs(e["top"]) + 2 * e["big"][:, None], 0)
+    close(o.top_log_prob, e["top"][index], t[index], "top_log_prob")
+    close(o.log_z, e["log_z"][index], e["tol_z"][index], "log_z")
+    close(o.entropy, e["entropy"][index], e["tol_h"][index], "entropy")
+
+
+@pytest.mark.parametrize("R, n", [(1, 49151), (1, 49152), (3, 49153), (127, 49152), (128, 49152), (40, 60001)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_on_both_sides_of_a_cut(R, n, dtype):
+    x, a, m = head(R, n, dtype, n)
+    if R > 2:
+        m[1], x[2, n // 3:] = False, -math.inf
+    check(x, a, m, 0.8, top=6)
+
+
+def test_two_streams_at_once():
+    """Calls that cut their rows have a workspace each."""
+    from muzero_amd.policy import policy_log_probs
+    sets = [head(5, 70001 + i, torch.bfloat16, i) for i in range(2)]
+    want = [policy_log_probs(x, a, mask=m, top=9) for x, a, m in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(10):
+        for i, (s, (x, a, m)) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(s):
+                got[i].append(policy_log_probs(x, a, mask=m, top=9))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        for o in outs:
+            assert all(torch.equal(p, q) for p, q in zip(w, o))
+
+
+def test_backward_twice_and_of_parts():
+    from muzero_amd.policy import policy_log_probs
+    x, a, m = head(7, 300, torch.float32, 1)
+    leaf = x.clone().requires_grad_()
+    out = policy_log_probs(leaf, a, mask=m, top=2)
+    one, = torch.autograd.grad(out.entropy.sum(), leaf, retain_graph=True)
+    two, = torch.autograd.grad(out.log_prob.sum(), leaf, retain_graph=True)
+    again, = torch.autograd.grad(out.entropy.sum(), leaf)
+    assert torch.equal(one, again) and not torch.equal(one, two)
+    out = policy_log_probs(leaf, a, mask=m)
+    graph, = torch.autograd.grad(out.log_z.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):                           # once differentiable: refused, not silently wrong
+        graph.sum().backward()

@@ -23,12 +23,12 @@ def adamw64(w, m, v, g, t, lr, wd, max_norm, b1=0.9, b2=0.999, eps=1e-8):
     return w * (1 - lr * wd) - lr / (1 - b1 ** t) * m / (np.sqrt(v / (1 - b2 ** t)) + eps)
 
 
-def trainer(fixture, **kw):
+def trainer(fixture, precision=None, **kw):
     from muzero_amd.engine import SearchEngine
     from muzero_amd.train import Trainer
     fx = load_golden(fixture + ".npz")
     dims = tuple(int(x) for x in fx["dims"])
-    dims = dims + (2,) if "vis" in fixture else dims
+    dims = dims + (2,) if "vis" in fixture else dims + (0, precision) if precision else dims
     eng = SearchEngine(dims, max_games=4, max_simulations=0)
     eng.set_weights(fx["blob0"])
     return fx, eng, Trainer(eng, int(fx["K"]), int(fx["B"]), "adamw", 0.01, **kw)
@@ -69,16 +69,16 @@ def test_trainer_steps(fixture, max_norm):
     eng.close()
 
 
-@pytest.mark.parametrize("fixture", ["train_tag123_K5_B128", "train_lstmB_K3_B32", "train_visB_K2_B4"])
-def test_inference_follows_the_trainer(fixture):
+@pytest.mark.parametrize("fixture, precision", [("train_tag123_K5_B128", None), ("train_tag123_K5_B128", 1), ("train_tag123_K5_B128", 2),
+                                                ("train_lstmB_K3_B32", None), ("train_visB_K2_B4", None)])
+def test_inference_follows_the_trainer(fixture, precision):
     from muzero_amd.engine import SearchEngine
-    fx, eng, tr = trainer(fixture, max_grad_norm=1.0)
+    fx, eng, tr = trainer(fixture, precision, max_grad_norm=1.0)
     tr.grad.copy_(torch.randn(tr.grad.numel(), generator=torch.Generator().manual_seed(1)).abs() * 0.01)
     tr.apply()
     blob = tr.weights()
     assert np.count_nonzero(blob != fx["blob0"]) > 0.9 * blob.size
-    dims = tuple(int(x) for x in fx["dims"])
-    other = SearchEngine(dims + (2,) if "vis" in fixture else dims, max_games=4, max_simulations=0)
+    other = SearchEngine(eng.dims, max_games=4, max_simulations=0)
     other.set_weights(blob)
     if "vis" in fixture:
         from test_vision_train_oracle import step_inputs
@@ -88,6 +88,25 @@ def test_inference_follows_the_trainer(fixture):
     for x, y in zip(eng.initial_inference(obs), other.initial_inference(obs)):
         assert torch.equal(x, y)
     eng.close(), other.close()
+
+
+def test_trainer_follows_the_momentum_schedule():
+    """onecyclelr moves beta1 with the rate, of AdamW as of Adam."""
+    from muzero_amd.train import scheduled_lr, scheduled_momentum
+    fx, eng, tr = trainer("train_tag123_K5_B128", weight_decay=0.05, lr_scheduler="onecyclelr", num_of_epoch=20)
+    w = tr.weights().astype(np.float64)
+    m, v, beta = np.zeros_like(w), np.zeros_like(w), []
+    for t in range(1, 4):
+        grad = torch.randn(w.size, generator=torch.Generator().manual_seed(t)) * 0.01
+        tr.grad.copy_(grad)
+        lr, b1 = scheduled_lr("onecyclelr", 0.01, 20, t - 1), scheduled_momentum("onecyclelr", 20, t - 1)
+        beta.append(b1)
+        tr.apply()
+        w = adamw64(w, m, v, grad.double().numpy(), t, lr, 0.05, None, b1=b1)
+        # beta1 below 0.95 and three steps: bias corrections as before, averages over the same three gradients
+        assert np.all(np.abs(tr.weights() - w) <= t * (60 * U * 0.01 + 2 * U * np.abs(w)) + U * np.abs(w))
+    assert len(set(beta)) > 1
+    eng.close()
 
 
 def test_trainer_refusals():
