@@ -266,9 +266,11 @@ struct Rank {
     static __device__ __forceinline__ Key next(const Key* key, Key last) {
         Key best = 0u - last; /* nothing: key 0 */
         _Pragma("unroll") for (int j = 0; j < E; ++j) best = max(best, key[j] - last);
-        best = lanes_reduce<G>(best, [](Key a, Key b) { return max(a, b); });
+        best = lanes_reduce<G>(best, larger);
         return last == 0 ? 0 : best + last;
     }
+    static __device__ __forceinline__ Key larger(Key a, Key b) { return max(a, b); }
+    static __device__ __forceinline__ Key smaller(Key a, Key b) { return min(a, b); }
 };
 template <>
 struct Rank<float> {
@@ -285,6 +287,11 @@ struct Rank<float> {
     static __device__ __forceinline__ Key larger(Key a, Key b) { /* neither is ever NaN: fmax would make sure of it first */
         Key v;
         asm("v_max_f64 %0, %1, %2" : "=v"(v) : "v"(a), "v"(b));
+        return v;
+    }
+    static __device__ __forceinline__ Key smaller(Key a, Key b) {
+        Key v;
+        asm("v_min_f64 %0, %1, %2" : "=v"(v) : "v"(a), "v"(b));
         return v;
     }
     template <int G, int E>
@@ -370,12 +377,15 @@ __device__ __forceinline__ bool is_plain(const Row& p, const Slope& q) {
     return !q.empty && !is_huge(p, q.big) && fabsf(q.base) < kInf && fabsf(q.slope) < kInf;
 }
 
-/* Alternatives of a row whose team holds all its keys: the next one below the last, `top` times; the team's lanes write one each. */
+/* Alternatives of a row whose team holds all its keys: the next one below the last, `top` times; the team's lanes write one each.  Where
+ * many are asked of many lanes, each of which then has one of them or none as a rule, they are looked for among the lanes' four largest, and
+ * anew among all keys if a lane's four were all taken (40000 x 1000 fp32 with 32 of them 217 -> 161 us, with 12 103 -> 76; 80000 x 1000 bf16
+ * with 32 233 -> 191, with 9 109 -> 101; fewer are not worth the sorting). */
 template <typename T, int kTeam, int E>
 __device__ __forceinline__ void write_best(const Row& p, int64_t r, int lane, const typename Rank<T>::Key* key, const Sum& v, const Values& o) {
     typename Rank<T>::Key last = Rank<T>::first(), mine = last;
-    int k = 0;
-    if (kTeam == 1) { /* four to a store: 2M rows of 8 with all 8 of them 66 us, one at a time 98 */
+    int k = 0; /* chosen already */
+    if constexpr (kTeam == 1) { /* four to a store: 2M rows of 8 with all 8 of them 66 us, one at a time 98 */
         for (; k + 4 <= p.top; k += 4) {
             w4_any at, lp;
             _Pragma("unroll") for (int i = 0; i < 4; ++i) {
@@ -387,12 +397,30 @@ __device__ __forceinline__ void write_best(const Row& p, int64_t r, int lane, co
             *reinterpret_cast<w4_any*>(p.top_log_prob + r * p.top + k) = lp;
         }
     }
-    for (; k < p.top; ++k) {
-        last = Rank<T>::template next<kTeam, E>(key, last);
-        const int turn = k % kTeam;
-        if (turn == lane) mine = last;
-        if ((turn == kTeam - 1 || k + 1 == p.top) && lane <= turn) write_top(p, r, k - turn + lane, Rank<T>::whole(mine), v, o);
+    const auto choose = [&](const auto& keys, auto count) {
+        for (int i = k; i < p.top; ++i) {
+            last = Rank<T>::template next<kTeam, decltype(count)::value>(keys, last);
+            const int turn = i % kTeam;
+            if (turn == lane) mine = last;
+            if ((turn == kTeam - 1 || i + 1 == p.top) && lane <= turn) write_top(p, r, i - turn + lane, Rank<T>::whole(mine), v, o);
+        }
+    };
+    if constexpr (kTeam >= 32 && E >= 12) {
+        if (p.top > 8 && 2 * p.top <= kTeam) {
+            typename Rank<T>::Key own[4] = {}; /* the lane's four largest */
+            _Pragma("unroll") for (int j = 0; j < E; ++j) {
+                typename Rank<T>::Key x = key[j];
+                _Pragma("unroll") for (int h = 0; h < 4; ++h) {
+                    const typename Rank<T>::Key large = Rank<T>::larger(own[h], x);
+                    x = Rank<T>::smaller(own[h], x), own[h] = large;
+                }
+            }
+            choose(own, std::integral_constant<int, 4>());
+            if (lanes_reduce<kTeam>(own[3] != 0 && own[3] >= last ? 1u : 0u, [](uint32_t a, uint32_t b) { return a | b; }) == 0) return;
+            last = Rank<T>::first();
+        }
     }
+    choose(key, std::integral_constant<int, E>());
 }
 
 /* ------------------------------------------------------------------ narrow rows
