@@ -101,7 +101,8 @@ class AdamW:
 
     state_bits 32: fp32 moments.  8: the first moment and the root of the second as e4m3 codes, one power-of-two exponent per 32 elements,
     rounded up or down by a counter-based dither from `seed` (2.06 bytes per parameter instead of 8).
-    master_weights: fp32 copies of bf16 / fp16 parameters are what the step updates; the parameters are their roundings.
+    master_weights: fp32 copies of bf16 / fp16 parameters are what the step updates; the parameters are their roundings, so
+    values written into the parameters afterwards last until the next step unless they go into state_tensors()["master"] too.
     max_grad_norm: gradients are scaled so that their global norm is at most that; a norm that is not finite skips the step.
 
     The step counter is on the device: a captured step() replays as the steps that follow.  lr may be a float or a 0-d
