@@ -9,6 +9,7 @@
  * of the type's lowest values (a mask written as numbers) has differences of 0, where c l_i would overflow.
  */
 #include "mzs_error.h"
+#include "mzs_policy_plan.h"
 
 #include <cstdint>
 
@@ -200,7 +201,7 @@ __device__ __forceinline__ float key_value(uint64_t key) {
     return __uint_as_float((b & 0x80000000u) ? b & 0x7fffffffu : ~b);
 }
 
-constexpr int kBlock = 256;
+constexpr int kBlock = kPolicyBlock;
 constexpr float kInf = __builtin_inff();
 
 /* a value of another lane, word by word */
@@ -500,7 +501,7 @@ __device__ __forceinline__ Sum team_merge(const Row& p, Sum v, float* lds) {
     return o;
 }
 
-constexpr int kAhead = 4; /* vectors a thread has in flight */
+constexpr int kAhead = kPolicyAhead; /* vectors a thread has in flight */
 
 /* The compiler may not look behind this: a row held packed is unpacked anew in each pass over it, where it would otherwise keep every
  * unpacked value (twice the registers, which spill). */
@@ -579,8 +580,7 @@ struct TopScratch {
 /* order of logits as unsigned numbers, 0 for what is not allowed */
 __device__ __forceinline__ uint32_t rank_value(float x) { return x == -kInf ? 0u : (uint32_t)(rank_key(x, 0) >> 32); }
 
-constexpr int kStripLanes = 4;                     /* neighbouring threads whose vectors make a strip */
-constexpr int kStripsPerBlock = kBlock / kStripLanes;
+constexpr int kStripLanes = kPolicyStripLanes, kStripsPerBlock = kPolicyStrips;
 constexpr int kHold = 16; /* strips of a row that a thread holds in registers */
 /* strip in held[h] of this thread; >= n_strips: none.  Few strips are spread over the block, so that every group has one. */
 __device__ __forceinline__ int held_strip(int h, int n_strips) {
@@ -1032,27 +1032,6 @@ Row pack(const mzs_policy_args& a) {
 /* widest row whose gradient sums the row again in registers rather than read its statistics back */
 constexpr int64_t kRegainMost = 2048;
 
-/* How a wide row is cut: `chunks` blocks a row, each thread `vecs` vectors.  Only few and long rows are: a block alone reads 12000 bf16 a us,
- * and the join costs a launch and a second search (us whole / cut, without alternatives and with five, logits from memory: 8 x 100000 bf16
- * - and 15 / 10, 64 of them 13 / 11 and 17 / 15, 100 13 / 13, 160 16 / 19 and 20 / 23; 8 x 50000 - and 10 / 10; 8 x 20000 - and 7.7 / 9.7, 64 5.5 / 6.9
- * and 8.4 / 11; fp32 32 x 100000 19 / 18 with, one of 30000 8 / 9). */
-struct Cut {
-    int chunks, vecs;
-};
-constexpr int64_t kCutLeast = 49152;
-Cut cut_row(int64_t rows, int64_t n, int per) {
-    const int64_t all = (n + (int64_t)kBlock * per - 1) / ((int64_t)kBlock * per); /* vectors a thread would have of a whole row */
-    int64_t chunks = 1;
-    if (rows < MZS_POLICY_MANY && n >= kCutLeast) chunks = (8192 + rows - 1) / rows;
-    if (chunks > kBlock) chunks = kBlock;
-    if (chunks > all) chunks = all;
-    Cut c;
-    c.vecs = (int)((all + chunks - 1) / chunks);
-    if (chunks > 1 && c.vecs > kAhead) c.vecs = (c.vecs + kAhead - 1) / kAhead * kAhead; /* whole groups */
-    c.chunks = (int)((all + c.vecs - 1) / c.vecs);
-    return c;
-}
-
 template <typename T, bool kForward, bool kGrad, bool kTop>
 void launch_lanes(const Row& p, hipStream_t st) {
     const int64_t blocks = (p.rows + kBlock - 1) / kBlock;
@@ -1062,13 +1041,12 @@ void launch_lanes(const Row& p, hipStream_t st) {
 }
 
 template <typename T>
-void launch_forward(const Row& p, const mzs_policy_args& a, hipStream_t st) {
-    const Cut c = cut_row(p.rows, p.n, Kind<T>::kPer);
+void launch_forward(const Row& p, const PolicyCut& c, void* workspace, hipStream_t st) {
     if (c.chunks == 1) {
         hipLaunchKernelGGL((k_policy_chunk<T, false>), dim3((unsigned)p.rows), dim3(kBlock), 0, st, p, 1, c.vecs, nullptr, nullptr);
         return;
     }
-    float* parts = static_cast<float*>(a.workspace);
+    float* parts = static_cast<float*>(workspace);
     float* strips = parts + 3 * p.rows * c.chunks;
     hipLaunchKernelGGL((k_policy_chunk<T, true>), dim3((unsigned)(p.rows * c.chunks)), dim3(kBlock), 0, st, p, c.chunks, c.vecs, parts, strips);
     hipLaunchKernelGGL(k_policy_join<T>, dim3((unsigned)p.rows), dim3(kBlock), 0, st, p, c.chunks, c.vecs, (const float*)parts,
@@ -1087,10 +1065,8 @@ void launch_slope(const Row& p, hipStream_t st) {
     }
 }
 
-/* rows in registers: up to kWaveVecs vectors a lane of a wave, kRowVecs a thread of a block of kRowThreads */
-constexpr int kRowThreads = 512, kWaveVecs = 16, kRowVecs = 24;
-template <typename T>
-bool fits_wave(int64_t n) { return n >= Kind<T>::kPer && n <= (int64_t)64 * kWaveVecs * Kind<T>::kPer; }
+/* rows in registers: up to kPolicyWaveVecs vectors a lane of a wave, kRowVecs a thread of a block of kRowThreads */
+constexpr int kRowThreads = 512, kRowVecs = 24;
 template <typename T>
 bool fits_block(int64_t n) { return n <= (int64_t)kRowThreads * kRowVecs * Kind<T>::kPer; }
 template <typename T, bool kGrad>
@@ -1167,8 +1143,6 @@ void launch_block_row(const Row& p, hipStream_t st) {
     else go(k_policy_row<T, kRowThreads, kRowVecs, true>);
 }
 
-constexpr int64_t kSlab = 1 << 20; /* rows of a launch: blocks times threads stay below 2^32 */
-
 /* rows [r, r + rows) of a call */
 template <typename T>
 Row rows_from(Row p, int64_t r, int64_t rows) {
@@ -1189,30 +1163,29 @@ Row rows_from(Row p, int64_t r, int64_t rows) {
  *   up to 24 vectors a thread   forward and gradient of a row in a block's registers        k_policy_row, a block
  *   beyond                      chunks and their join; the gradient from the statistics     k_policy_chunk, k_policy_join, k_policy_slope */
 template <typename T>
-void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool forward, bool grad) {
-    const bool wave = fits_wave<T>(all.n) && all.n > 8, lanes = all.n <= 8;
-    const int64_t slab = wave || lanes ? (int64_t)1 << 24 : kSlab;
-    for (int64_t r = 0; r < all.rows; r += slab) {
-        const Row p = rows_from<T>(all, r, all.rows - r < slab ? all.rows - r : slab);
-        const bool both = forward && grad && p.top == 0;
+void run_kind(const Row& all, const PolicyPlan& plan, void* workspace, hipStream_t st, bool forward, bool grad) {
+    const bool lanes = all.n <= kPolicyLanesMost, wave = !lanes && policy_fits_wave(all.n, Kind<T>::kPer);
+    const bool both = forward && grad && all.top == 0;
+    policy_launches(all.rows, plan, [&](int64_t first, int64_t rows, const PolicyPlan&) {
+        const Row p = rows_from<T>(all, first, rows);
         if (both && wave) {
             launch_wave_row<T, true>(p, st);
-            continue;
+            return;
         }
         if (both && lanes) {
             launch_lanes<T, true, true, false>(p, st);
-            continue;
+            return;
         }
         if (both && fits_block<T>(p.n)) {
             launch_block_row<T>(p, st);
-            continue;
+            return;
         }
         if (forward) {
             if (wave && p.top == 0) launch_wave_row<T, false>(p, st);
             else if (wave && p.n <= kRankMost) launch_wave_top<T>(p, st);
             else if (lanes && p.top > 0) launch_lanes<T, true, false, true>(p, st);
             else if (lanes) launch_lanes<T, true, false, false>(p, st);
-            else launch_forward<T>(p, a, st);
+            else launch_forward<T>(p, plan.cut, workspace, st);
         }
         if (grad) {
             Row g = p;
@@ -1221,30 +1194,24 @@ void run_kind(const Row& all, const mzs_policy_args& a, hipStream_t st, bool for
             else if (lanes) launch_lanes<T, false, true, false>(p, st);
             else launch_slope<T>(p, st);
         }
-    }
+    });
 }
 
-size_t workspace_bytes(const mzs_policy_args& a, int per) {
-    if (a.rows == 0 || a.n_actions <= MZS_POLICY_NARROW) return 0;
-    const Cut c = cut_row(a.rows, a.n_actions, per);
-    if (c.chunks == 1) return 0;
-    return sizeof(float) * (size_t)a.rows * c.chunks * (3 + (a.top > 0 ? kStripsPerBlock : 0));
-}
+PolicyPlan plan_of(const mzs_policy_args& a) { return policy_plan(a.rows, a.n_actions, a.dtype == MZS_DTYPE_FLOAT ? 4 : 8, a.top); }
 
 int run(const mzs_policy_args* a, void* stream, bool forward, bool grad) {
     const int rc = check(a, forward, grad);
     if (rc || a->rows == 0) return rc;
-    if (forward) {
-        const size_t need = workspace_bytes(*a, a->dtype == MZS_DTYPE_FLOAT ? 4 : 8);
-        if (need && (!a->workspace || a->workspace_bytes < need)) return set_error(MZS_E_ARG, "workspace too small (mzs_policy_workspace)");
-    }
+    const PolicyPlan plan = plan_of(*a);
+    if (forward && plan.workspace && (!a->workspace || a->workspace_bytes < plan.workspace))
+        return set_error(MZS_E_ARG, "workspace too small (mzs_policy_workspace)");
     DeviceScope scope(a->device);
     if (scope.status != hipSuccess) return hip_error("mzs_policy: device", scope.status);
     const Row p = pack(*a);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a->dtype == MZS_DTYPE_FLOAT) run_kind<float>(p, *a, st, forward, grad);
-    else if (a->dtype == MZS_DTYPE_BFLOAT) run_kind<__bf16>(p, *a, st, forward, grad);
-    else run_kind<_Float16>(p, *a, st, forward, grad);
+    if (a->dtype == MZS_DTYPE_FLOAT) run_kind<float>(p, plan, a->workspace, st, forward, grad);
+    else if (a->dtype == MZS_DTYPE_BFLOAT) run_kind<__bf16>(p, plan, a->workspace, st, forward, grad);
+    else run_kind<_Float16>(p, plan, a->workspace, st, forward, grad);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? MZS_OK : hip_error("mzs_policy: launch", e);
 }
@@ -1258,7 +1225,7 @@ int mzs_policy_workspace(const mzs_policy_args* args, size_t* bytes_out) {
     if (!args || !bytes_out) return mzs::set_error(MZS_E_ARG, "null argument");
     if (args->dtype < MZS_DTYPE_FLOAT || args->dtype > MZS_DTYPE_HALF || args->rows < 0 || args->n_actions < 1 || args->n_actions > (1 << 28))
         return mzs::set_error(MZS_E_ARG, "fp32, bf16 or fp16; rows >= 0 and 1 <= n_actions <= 2^28");
-    *bytes_out = mzs::workspace_bytes(*args, args->dtype == MZS_DTYPE_FLOAT ? 4 : 8);
+    *bytes_out = args->rows ? mzs::plan_of(*args).workspace : 0;
     return MZS_OK;
 }
 int mzs_policy_log_probs(const mzs_policy_args* args, void* stream) { return mzs::run(args, stream, true, false); }

@@ -1,10 +1,14 @@
 """Policy rows and optimizer, host side: what the C-ABI and the Python wrappers refuse without a GPU."""
 import ctypes as C
+import os
+import subprocess
 
 import pytest
 import torch
 
 from muzero_amd import _lib, optim, policy
+
+HERE = os.path.dirname(os.path.abspath(__file__))
 
 
 def args(**kw):
@@ -111,3 +115,38 @@ def test_wrappers_refuse_host_tensors_and_bad_types():
         optim.grad_norm([x, x.double()])
     with pytest.raises(ValueError, match="contiguous"):
         optim.grad_norm([torch.zeros(4, 4).t()[1:]])
+
+
+def plan_check(tmp_path, calls):
+    """(launches, workspace bytes, chunks a row) of each call [rows, logits, logits per vector, top]; the program fails on a plan whose launches
+    need more workspace than the call was told."""
+    exe = tmp_path / "policy_plan_check"
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-o", str(exe), os.path.join(HERE, "csrc", "policy_plan_check.cpp")])
+    out = subprocess.run([str(exe), *(str(v) for c in calls for v in c)], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0, out.stdout
+    return [tuple(int(v) for v in line.split()) for line in out.stdout.splitlines()[:-1]]
+
+
+def test_every_launch_of_a_call_follows_the_call_s_plan(tmp_path):
+    """Rows around 128 (fewer are cut) and around whole launches, whose rest must not be cut by itself."""
+    rows = [k * 2 ** 20 + r for k in (0, 1, 2, 16, 17) for r in (0, 1, 2, 5, 40, 127, 128, 129, 2 ** 20 - 1) if k or r]
+    calls = [(r, n, per, top) for r in rows for n in (1, 8, 9, 2048, 2049, 4096, 4097, 8192, 8193, 49151, 49152, 50000, 2 ** 20, 2 ** 28)
+             for per in (4, 8) for top in (0, 5)]
+    plans = plan_check(tmp_path, calls)
+    assert max(p[0] for p in plans) > 16 and max(p[2] for p in plans) == 256
+    lib, size = _lib.load(), C.c_size_t()
+    for (r, n, per, top), (_, workspace, _) in zip(calls, plans):
+        a = args(rows=r, n_actions=n, dtype=_lib.DTYPE_FLOAT if per == 4 else _lib.DTYPE_HALF, top=top)
+        assert lib.mzs_policy_workspace(C.byref(a), C.byref(size)) == 0 and size.value == workspace
+        if n <= _lib.POLICY_NARROW or r >= _lib.POLICY_MANY:
+            assert workspace == 0
+
+
+def test_a_cut_call_without_its_workspace_is_refused():
+    lib = _lib.load()
+    a = args(rows=5, n_actions=50000, logits_stride=0, dtype=_lib.DTYPE_BFLOAT)
+    size = C.c_size_t()
+    assert lib.mzs_policy_workspace(C.byref(a), C.byref(size)) == 0 and size.value > 0
+    for given, at in ((0, None), (size.value - 1, 4096), (size.value, None)):
+        a.workspace, a.workspace_bytes = at, given
+        assert lib.mzs_policy_log_probs(C.byref(a), None) == -1 and b"workspace" in lib.mzs_last_error()
