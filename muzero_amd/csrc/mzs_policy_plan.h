@@ -53,10 +53,11 @@ inline size_t policy_launch_bytes(const PolicyCut& c, int64_t rows, int top) { /
     return c.chunks == 1 ? 0 : sizeof(float) * (size_t)rows * c.chunks * (3 + (top > 0 ? kPolicyStrips : 0));
 }
 inline PolicyPlan policy_plan(int64_t rows, int64_t n, int per, int top) {
-    const bool narrow = n <= kPolicyLanesMost || policy_fits_wave(n, per);
     PolicyPlan p;
     p.cut = policy_cut(rows, n, per);
-    p.slab = narrow ? (int64_t)1 << 24 : (int64_t)1 << 20; /* blocks times threads stay below 2^32 */
+    /* blocks times threads stay below 2^32: a wave a row at most, or a block, which a row that a wave could hold gets for its
+     * alternatives and its gradient */
+    p.slab = n <= MZS_POLICY_NARROW ? (int64_t)1 << 24 : (int64_t)1 << 20;
     p.workspace = policy_launch_bytes(p.cut, rows, top);
     return p;
 }

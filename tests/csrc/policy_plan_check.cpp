@@ -20,6 +20,7 @@ int main(int argc, char** argv) {
             bad += c.chunks != call.cut.chunks || c.vecs != call.cut.vecs;
             bad += c.chunks < 1 || c.chunks > mzs::kPolicyBlock;                    /* a thread of the join each */
             bad += (c.chunks * chunk < n || (c.chunks - 1) * chunk >= n);   /* the chunks are the row, none is empty */
+            bad += n > MZS_POLICY_NARROW && count * c.chunks * mzs::kPolicyBlock >= (int64_t)1 << 32; /* a block a row */
             next = first + count, ++launches;
         });
         bad += next != rows;

@@ -98,3 +98,15 @@ def test_more_wide_rows_than_a_launch_takes(n):
         check_rows(at_borders(rows, 2 ** 20), x, a, m, 1.3, top, out, up, grad)
         assert bool((out.log_z == out.log_z[0]).all())
         del out, grad
+
+
+def test_a_block_a_row_for_more_rows_than_blocks_of_a_launch():
+    """2^24 + 5 rows of 2049: a wave could hold them, their alternatives are looked for by a block each."""
+    from muzero_amd.policy import policy_log_probs
+    rows, n = 2 ** 24 + 5, 2049
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(1, n, generator=g).half().cuda().expand(rows, n)
+    a = torch.randint(-1, n, (rows,), generator=g).cuda()
+    out = policy_log_probs(x, a, top=1)
+    check_rows(torch.cat([at_borders(rows, 2 ** 20), at_borders(rows, 2 ** 24)]), x, a, None, 1.0, 1, out)
+    assert bool((out.log_z == out.log_z[0]).all()) and bool((out.top_action == out.top_action[0]).all())
