@@ -303,9 +303,11 @@ struct Rank<float> {
     }
 };
 
-/* c * big overflows, or its products lose the differences: such rows (the type's lowest values as a mask, all of them; 1e30 and
- * more) take their exponents as c (l_i - big) */
-constexpr float kHuge = 1e30f;
+/* From |c big| = kHuge on a row takes its exponents as c (l_i - big).  Below, they are c l_i - m with one rounding, m = c big rounded, and
+ * delta = c big - m, at most half a step of m, is put right by 2^-delta: that has to stay near 1, and is, up to 2^24 (delta <= 1/2), where it
+ * would be 0 or infinity from 2^34 on.  Rows up there are those of large numbers written as a mask (-1e9 everywhere) or of temperatures
+ * below about 1e-6. */
+constexpr float kHuge = 0x1p24f;
 __device__ __forceinline__ bool is_huge(const Row& p, float big) { return !(fabsf(p.c * big) < kHuge); }
 
 /* exponent of 2 for a logit x beside the row's largest one; finite, so that 0 * it is 0 */
@@ -513,18 +515,21 @@ __device__ __forceinline__ float max_vecs(const w4* v, float big) {
         _Pragma("unroll") for (int j = 0; j < Kind<T>::kPer; ++j) big = fmaxf(big, Kind<T>::get(v[u], j));
     return big;
 }
-/* A thread's running sum over the vectors of a wide row, relative to m = c * big held within +-kHuge: the exponent is one fma, c l_i - m
- * with a single rounding, and what m lost to its own rounding is put right once at the end.  Where m was held, nothing is
- * allowed yet (all exponentials are 0) or the row is huge: then the chunk is summed again by sum_slowly. */
+/* A thread's running sum over the vectors of a wide row, relative to m = c * big held within +-kReach: the exponent is one fma, c l_i - m
+ * with a single rounding, and what m lost to its own rounding is put right once at the end.  Where m was held above, the row is huge and
+ * summed again by sum_slowly; where it was held below, either all of the row is as low and huge too, or the row's largest logit is at least
+ * 2^24 above in exponents and what this thread has counts for nothing (kReach is twice kHuge for that: a part that lies a little below
+ * a row that is just not huge still has its own m). */
+constexpr float kReach = 2.0f * kHuge;
 struct Running {
     float big, m, s, t;
 };
-__device__ __forceinline__ Running running_start() { return Running{-kInf, -kHuge, 0.0f, 0.0f}; }
+__device__ __forceinline__ Running running_start() { return Running{-kInf, -kReach, 0.0f, 0.0f}; }
 
 /* takes N vectors: their maximum first, one rescaling, then the exponentials */
 template <typename T, int N>
 __device__ __forceinline__ void take_vecs(const Row& p, const w4* v, Running& sum) {
-    const float big = max_vecs<T, N>(v, sum.big), m = __builtin_amdgcn_fmed3f(p.c * big, -kHuge, kHuge);
+    const float big = max_vecs<T, N>(v, sum.big), m = __builtin_amdgcn_fmed3f(p.c * big, -kReach, kReach);
     const float shift = fmaxf(sum.m - m, kLow), f = __builtin_amdgcn_exp2f(shift);
     float s = f * sum.s, t = f * (sum.t + shift * sum.s);
     _Pragma("unroll") for (int u = 0; u < N; ++u)
@@ -536,14 +541,14 @@ __device__ __forceinline__ void take_vecs(const Row& p, const w4* v, Running& su
 }
 /* takes one logit */
 __device__ __forceinline__ void take_one(const Row& p, float x, Running& sum) {
-    const float big = fmaxf(sum.big, x), m = __builtin_amdgcn_fmed3f(p.c * big, -kHuge, kHuge);
+    const float big = fmaxf(sum.big, x), m = __builtin_amdgcn_fmed3f(p.c * big, -kReach, kReach);
     const float shift = fmaxf(sum.m - m, kLow), f = __builtin_amdgcn_exp2f(shift);
     const float d = fmaf(p.c, x, -m), e = __builtin_amdgcn_exp2f(d);
     sum = Running{big, m, f * sum.s + e, fmaf(e, fmaxf(d, kLow), f * (sum.t + shift * sum.s))};
 }
-/* the same relative to big itself */
+/* the same relative to big itself, where m was not held */
 __device__ __forceinline__ Sum running_end(const Row& p, const Running& v) {
-    const float delta = is_huge(p, v.big) ? 0.0f : fmaf(p.c, v.big, -v.m), f = __builtin_amdgcn_exp2f(-delta);
+    const float delta = fabsf(v.m) < kReach ? fmaf(p.c, v.big, -v.m) : 0.0f, f = __builtin_amdgcn_exp2f(-delta);
     return Sum{v.big, f * v.s, f * (v.t - delta * v.s)};
 }
 /* this thread's vectors i, i + stride, ... and its extra logit (-inf: none) of a row whose largest logit `big` is huge */
