@@ -175,6 +175,10 @@ int32_t mzs_hidden_stride(const mzs_handle* h);
 int mzs_initial_inference(mzs_handle* h, int32_t batch, const float* obs_dev, float* hidden_dev,
                           float* policy_dev, float* value_dev, void* stream);
 
+/* The same with the policy head's logits [B][A] instead of their softmax, whose exponentials end at e^-87. */
+int mzs_initial_logits(mzs_handle* h, int32_t batch, const float* obs_dev, float* hidden_dev,
+                       float* logits_dev, void* stream);
+
 /* Muzero.dynamics_function_inference + prediction_function_inference on the new state
  * (muzero_model.py:848-905): reward [B], next_hidden [B][S_dim], policy [B][A], value [B].
  * policy/value may be NULL (dynamics only). */

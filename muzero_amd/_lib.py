@@ -102,6 +102,7 @@ _SIGNATURES = {
     "mzs_hidden_stride": (C.c_int32, [C.c_void_p]),
     "mzs_initial_inference": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
                                         C.c_void_p, C.c_void_p]),
+    "mzs_initial_logits": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "mzs_recurrent_inference": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                           C.c_void_p]),

@@ -495,14 +495,14 @@ __device__ __forceinline__ float model_dynamics(const Model& m, const WaveLds& L
     return reward;
 }
 
-/* Prediction_function.forward on L.xh: softmax policy as lane pairs, value (uniform) */
-template <bool kVision, int kVisBatch = 64>
+/* Prediction_function.forward on L.xh: softmax policy (kLogits: its logits) as lane pairs, value (uniform) */
+template <bool kVision, int kVisBatch = 64, bool kLogits = false>
 __device__ __forceinline__ float model_prediction(const Model& m, const WaveLds& L, Pair* policy,
                                                   int lane) {
-    if constexpr (kVision) return vis_prediction<kVisBatch>(m, L, policy, lane);
+    if constexpr (kVision) return vis_prediction<kVisBatch, kLogits>(m, L, policy, lane);
     if (m.kind == MZS_MODEL_LSTM) {
         const float* pl = lstm_head(m, m.l_pol, L, L.xh, -1, lane);
-        *policy = seg_softmax(seg_load(pl, m.A, lane));
+        *policy = kLogits ? seg_load(pl, m.A, lane) : seg_softmax(seg_load(pl, m.A, lane));
         wave_sync();
         const float* vl = lstm_head(m, m.l_val, L, L.xh, -1, lane);
         return seg_support_scalar(vl, m.Sd, lane);
@@ -510,7 +510,7 @@ __device__ __forceinline__ float model_prediction(const Model& m, const WaveLds&
     wave_dense<true>(m.w, m.p_in, L.xh, L.xa, -1, lane, m.bf16);
     float* t = wave_mid_layers(m, m.p_mid, L.xa, L.xb, lane);
     wave_dense<false>(m.w, m.p_heads, t, L.ob, -1, lane, m.bf16);
-    *policy = seg_softmax(seg_load(L.ob, m.A, lane));
+    *policy = kLogits ? seg_load(L.ob, m.A, lane) : seg_softmax(seg_load(L.ob, m.A, lane));
     return seg_support_scalar(L.ob + m.seg_value, m.Sd, lane);
 }
 

@@ -505,8 +505,8 @@ __device__ __forceinline__ float vis_dynamics(const Model& m, const WaveLds& L, 
     return reward;
 }
 
-/* hidden state in L.xh (kept) -> softmax policy as lane pairs, value (uniform) */
-template <int NB = 64>
+/* hidden state in L.xh (kept) -> softmax policy (kLogits: its logits) as lane pairs, value (uniform) */
+template <int NB = 64, bool kLogits = false>
 __device__ __forceinline__ float vis_prediction(const Model& m, const WaveLds& L, Pair* policy, int lane) {
     const mzs_vision_offsets o = vis_offsets(m);
     const float* __restrict__ blob = m.blob;
@@ -525,7 +525,7 @@ __device__ __forceinline__ float vis_prediction(const Model& m, const WaveLds& L
             wave_sync();
         }
     }
-    *policy = seg_softmax(seg_load(logits, m.A, lane));
+    *policy = kLogits ? seg_load(logits, m.A, lane) : seg_softmax(seg_load(logits, m.A, lane));
     wave_sync();
     return value;
 }

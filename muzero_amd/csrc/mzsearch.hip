@@ -386,14 +386,14 @@ struct InferParams {
     const int* action;     /* [B]                                */
     float* reward;         /* [B]                                */
     float* hidden_out;     /* [B][hid]                           */
-    float* policy;         /* [B][A]                             */
+    float* policy;         /* [B][A] (kLogits: the softmax's logits) */
     float* value;          /* [B]                                */
     long long hidden_stride; /* floats between the rows of hidden_out (0: hid) */
 };
 
 enum { kInferInitial = 0, kInferRecurrent = 1, kInferPrediction = 2 };
 
-template <int kMode, bool kVision = false>
+template <int kMode, bool kVision = false, bool kLogits = false>
 __global__ void __launch_bounds__(256) k_inference(const InferParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = lane_id();
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(256) k_inference(const InferParams p) {
     }
     if (p.policy || p.value) {
         Pair pol;
-        const float value = model_prediction<kVision>(m, L, &pol, lane);
+        const float value = model_prediction<kVision, 64, kLogits>(m, L, &pol, lane);
         if (p.policy) pair_to_global(p.policy + (size_t)b * m.A, pol, lane);
         if (p.value && lane == 0) p.value[b] = value;
     }
@@ -1754,7 +1754,7 @@ int32_t mzs_hidden_stride(const mzs_handle* h) { return h ? h->tree.hid_stride :
 
 static int run_inference(mzs_handle* h, int mode, int32_t batch, const float* in,
                          const int32_t* action, float* reward, float* hidden_out, float* policy,
-                         float* value, void* stream) {
+                         float* value, void* stream, bool logits = false) {
     if (!h) return fail(MZS_E_ARG, "null handle");
     if (!h->have_weights) return fail(MZS_E_STATE, "mzs_set_weights has not been called");
     if (batch < 0 || !in) return fail(MZS_E_ARG, "bad batch or null input");
@@ -1774,6 +1774,10 @@ static int run_inference(mzs_handle* h, int mode, int32_t batch, const float* in
     p.policy = policy;
     p.value = value;
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (logits) { /* initial inference only */
+        if (h->cfg.dims.model_kind == MZS_MODEL_VISION) return launch(k_inference<kInferInitial, true, true>, p, batch, p.lds, st);
+        return launch(k_inference<kInferInitial, false, true>, p, batch, p.lds, st);
+    }
     if (h->cfg.dims.model_kind == MZS_MODEL_VISION) {
         if (mode == kInferInitial) return launch(k_inference<kInferInitial, true>, p, batch, p.lds, st);
         if (mode == kInferRecurrent) return launch(k_inference<kInferRecurrent, true>, p, batch, p.lds, st);
@@ -1788,6 +1792,13 @@ int mzs_initial_inference(mzs_handle* h, int32_t batch, const float* obs_dev, fl
                           float* policy_dev, float* value_dev, void* stream) {
     return run_inference(h, kInferInitial, batch, obs_dev, nullptr, nullptr, hidden_dev, policy_dev,
                          value_dev, stream);
+}
+
+int mzs_initial_logits(mzs_handle* h, int32_t batch, const float* obs_dev, float* hidden_dev,
+                       float* logits_dev, void* stream) {
+    if (!logits_dev) return fail(MZS_E_ARG, "logits output is null");
+    return run_inference(h, kInferInitial, batch, obs_dev, nullptr, nullptr, hidden_dev, logits_dev,
+                         nullptr, stream, true);
 }
 
 int mzs_recurrent_inference(mzs_handle* h, int32_t batch, const float* hidden_dev,

@@ -335,6 +335,16 @@ class SearchEngine:
                                                   _ptr(val), self._stream()), "mzs_initial_inference")
         return hid, pol, val
 
+    def initial_logits(self, obs):
+        """The policy head's logits [B, A] of observations, which initial_inference returns as their softmax."""
+        obs = self._dev(obs, torch.float32)
+        B = obs.shape[0]
+        hid = torch.empty((B, self.hidden_floats), dtype=torch.float32, device=self.device)
+        logits = torch.empty((B, self.A), dtype=torch.float32, device=self.device)
+        _lib.check(self.lib.mzs_initial_logits(self.h, B, _ptr(obs), _ptr(hid), _ptr(logits), self._stream()),
+                   "mzs_initial_logits")
+        return logits
+
     def recurrent_inference(self, hidden, action, want_prediction=True):
         hidden = self._dev(hidden, torch.float32)
         action = self._dev(action, torch.int32)

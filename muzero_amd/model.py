@@ -407,14 +407,16 @@ class Muzero:
     def policy_statistics(self, states, actions=None, temperature=1.0, top=0):
         """The policy head on a batch of observations as PolicyLogProbs (muzero_amd.policy): the log-probability of
         `actions` (indices into action_dictionnary; None: 0), the entropy and the `top` most likely actions of
-        softmax(logits / temperature).  No counterpart in the reference (its inference returns the softmax alone,
-        muzero_model.py:883-905)."""
+        softmax(logits / temperature); log_z is that of the head's log-probabilities at `temperature` (0 at 1).  No
+        counterpart in the reference (its inference returns the softmax alone, muzero_model.py:883-905)."""
         from .policy import policy_log_probs
         obs = self._as_images(states) if self.is_RGB else self._as_batch(states)
-        _, pol, _ = self._inference_engine().initial_inference(obs)
+        logits = self._inference_engine().initial_logits(obs)
         if actions is not None:
-            actions = torch.as_tensor(actions).reshape(-1).to(device=pol.device, dtype=torch.int64)
-        return policy_log_probs(torch.log(pol), actions, temperature=temperature, top=top)
+            actions = torch.as_tensor(actions).reshape(-1).to(device=logits.device, dtype=torch.int64)
+        # not the logarithm of the softmax: its exponentials end at e^-87, and a smaller one may count at a temperature above 1
+        logits -= policy_log_probs(logits).log_z[:, None]
+        return policy_log_probs(logits, actions, temperature=temperature, top=top)
 
     def train(self, batch):
         """muzero_model.py:791-811: one optimizer step on `batch` = (samples, importance-sampling

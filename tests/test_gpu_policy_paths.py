@@ -259,3 +259,54 @@ def test_operators_together():
         for p, old, q, (m, v) in zip((w, b), before, grads, state):
             want = adamw64(old, m, v, q * min(1.0, 0.05 / (norm + 1e-6)), t, 0.01, 0.1, 0.0)
             assert np.all(np.abs(p.detach().cpu().numpy() - want) <= 60 * U * 0.01 * t + 3 * U * np.abs(want))
+
+
+@pytest.mark.parametrize("name, precision", [("tag123", 0), ("tag137", 0), ("lstmA", 0), ("visA", 0), ("tag123", 1)])
+def test_logits_of_the_policy_head(name, precision):
+    """Their softmax is initial_inference's policy: 3 roundings of the exponent, 8 of exponential, sum and quotient on each side."""
+    from conftest import fixture_weights
+    from muzero_amd.engine import SearchEngine
+    d, blob = fixture_weights(name)
+    obs = np.random.RandomState(3).uniform(-1, 1, size=(5, 3, 98, 98) if name == "visA" else (37, d.obs_dim)).astype(np.float32)
+    eng = SearchEngine((d.obs_dim, d.n_actions, d.state_dim, d.hidden_dim, d.n_mid_layers, d.model_kind, precision),
+                       max_games=len(obs), max_simulations=0)
+    eng.set_weights(blob)
+    logits, p = eng.initial_logits(obs).double(), eng.initial_inference(obs)[1].double()
+    want = torch.log_softmax(logits, 1)
+    assert float((want.exp() - p).abs().max()) <= (16 + 4 * float(logits.abs().max())) * U and float(logits.std()) > 0
+    eng.close()
+
+
+def test_model_statistics_of_a_head_that_is_sure():
+    """Policies with probabilities below e^-87, where the inference's softmax ends: they have a log-probability, and count at temperatures
+    above 1.  The policy head's weights 2^10 times as large give logits of exactly 2^10 times; u of the largest logit for each of their three
+    roundings behind it."""
+    from muzero_amd.model import Muzero
+    fx = load_golden("train_tag123_K5_B128.npz")
+    mz = Muzero(model_structure="mlp_model", observation_space_dimensions=4, action_space_dimensions=2, state_space_dimensions=31,
+                hidden_layer_dimensions=64, number_of_hidden_layer=0)
+    mz.set_weights(fx["blob0"])
+    obs = fx["s0_obs"][:33]
+    logits = mz._inference_engine().initial_logits(obs).double().cpu().numpy()
+    H, A, Sd = 64, 2, 31
+    blob = np.array(fx["blob0"])
+    # behind the representation, dynamics and the prediction's first layer: A x H weights and A biases of the policy
+    head = len(blob) - (A * H + A + Sd * H + Sd)
+    blob[head:head + A * H + A] *= 1024.0
+    mz.set_weights(blob)
+    sure = mz._inference_engine().initial_logits(obs).double().cpu().numpy()
+    assert np.array_equal(sure, 1024.0 * logits)
+    p = mz._inference_engine().initial_inference(obs)[1].cpu().numpy()
+    actions = np.argmin(sure, axis=1)
+    logs = sure - np.logaddexp.reduce(sure, axis=1)[:, None]
+    assert (np.log(p[np.arange(33), actions]) > logs[np.arange(33), actions] + 100.0).any()
+    for temperature in (1.0, 10.0, 300.0):
+        z = logs / temperature
+        lz = np.logaddexp.reduce(z, axis=1)
+        q = z - lz[:, None]
+        out = mz.policy_statistics(obs, actions, temperature=temperature, top=2)
+        tol = (32 + 8 * np.abs(sure).max() / temperature) * U
+        assert np.abs(out.log_prob.cpu().numpy() - q[np.arange(33), actions]).max() <= tol
+        assert np.abs(out.log_z.cpu().numpy() - lz).max() <= tol
+        assert np.abs(out.entropy.cpu().numpy() + (np.exp(q) * q).sum(1)).max() <= tol
+        assert np.array_equal(out.top_action.cpu().numpy(), np.argsort(-sure, axis=1, kind="stable"))
