@@ -106,8 +106,9 @@ class AdamW:
     max_grad_norm: gradients are scaled so that their global norm is at most that; a norm that is not finite skips the step.
 
     The step counter is on the device: a captured step() replays as the steps that follow.  lr may be a float or a 0-d
-    float32 tensor on the GPU (which a captured step reads at every replay).  Parameters whose gradient is None are
-    left as they are."""
+    float32 tensor on the GPU (which a captured step reads at every replay).  lr, betas, eps, weight_decay, max_grad_norm and
+    seed are read by every step() and may be changed between steps (a replayed step keeps those of its capture).
+    Parameters whose gradient is None are left as they are."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
                  master_weights=False, max_grad_norm=None, seed=0):
@@ -156,7 +157,6 @@ class AdamW:
         self._workspace = torch.empty(size, dtype=torch.uint8, device=dev)      # as the states, for one step at a time
         a.workspace, a.workspace_bytes = self._workspace.data_ptr(), size
         a.device, a.n, a.param_dtype, a.state_bits = dev.index, len(params), _DTYPES[params[0].dtype], state_bits
-        a.beta1, a.beta2, a.eps, a.weight_decay = self.betas[0], self.betas[1], eps, weight_decay
         a.exp_avg = self._state["exp_avg"].data_ptr()
         a.exp_avg_sq = self._state["exp_avg_sq" if state_bits == 32 else "exp_avg_root"].data_ptr()
         if state_bits == 8:
@@ -164,7 +164,7 @@ class AdamW:
             a.exp_avg_sq_exponent = self._state["exp_avg_root_exponent"].data_ptr()
         if master_weights:
             a.master = self._state["master"].data_ptr()
-        a.control_dev, a.seed = self.control.data_ptr(), self.seed & (2 ** 64 - 1)
+        a.control_dev = self.control.data_ptr()
 
     # ------------------------------------------------------------------ state
     def state_tensors(self):
@@ -200,7 +200,6 @@ class AdamW:
         self.control[0] = int(state["step"])
         if "seed" in state:
             self.seed = int(state["seed"])
-            self._args.seed = self.seed & (2 ** 64 - 1)
 
     def zero_grad(self):
         for p in self.params:
@@ -247,6 +246,8 @@ class AdamW:
         a = self._args
         a.n_tiles, a.params_table, a.grads_table = params_table.tiles, params_table.ptr, table.ptr
         a.grad_dtype, a.grad_scale = _DTYPES[dtype], float(grad_scale)
+        a.beta1, a.beta2 = self.betas
+        a.eps, a.weight_decay, a.seed = self.eps, self.weight_decay, self.seed & (2 ** 64 - 1)
         lr = self.lr
         if isinstance(lr, torch.Tensor):
             if lr.dtype is not torch.float32 or lr.device != self.device or lr.numel() != 1:

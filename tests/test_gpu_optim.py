@@ -497,3 +497,36 @@ def test_many_tensors_and_steps_on_a_side_stream():
     for _ in range(3):
         two.step(gs)
     assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_values_changed_between_steps_count(bits):
+    """Each step against a new optimizer with those values that goes on from the same state."""
+    from muzero_amd import _lib
+    from muzero_amd.optim import AdamW
+    sizes = [40, 5000]
+    a = make(sizes, torch.float32, 0, scale=1.0)
+    opt = AdamW(a, max_grad_norm=1.0, state_bits=bits)
+    opt.step(make(sizes, torch.float32, 1))
+    changes = (dict(betas=(0.5, 0.9)), dict(eps=1e-2), dict(weight_decay=0.5), dict(lr=0.1), dict(max_grad_norm=0.01), dict(seed=77),
+               dict(max_grad_norm=None))
+    values = dict(max_grad_norm=1.0)
+    for k, change in enumerate(changes):
+        values.update(change)
+        b = [p.clone() for p in a]
+        other = AdamW(b, state_bits=bits, **values)
+        other.load_state_dict({n: v for n, v in opt.state_dict().items() if n != "seed"})
+        before, g = [p.clone() for p in a], make(sizes, torch.float32, 2 + k)
+        for name, v in change.items():
+            setattr(opt, name, v)
+        opt.step(g), other.step(g)
+        assert all(torch.equal(p, q) for p, q in zip(a, b)) and not torch.equal(a[0], before[0])
+        for n, v in opt.state_tensors().items():
+            assert torch.equal(v.view(torch.uint8), other.state_tensors()[n].view(torch.uint8))
+    for name, bad in (("betas", (1.0, 0.9)), ("eps", -1.0), ("weight_decay", -0.1), ("lr", -1.0)):
+        keep = getattr(opt, name)
+        setattr(opt, name, bad)
+        with pytest.raises(_lib.MzsError):
+            opt.step(make(sizes, torch.float32, 1))
+        setattr(opt, name, keep)
+    assert opt.step_count == 1 + len(changes)
