@@ -108,12 +108,14 @@ class AdamW:
     The step counter is on the device: a captured step() replays as the steps that follow.  lr may be a float or a 0-d
     float32 tensor on the GPU (which a captured step reads at every replay).  lr, betas, eps, weight_decay, max_grad_norm and
     seed are read by every step() and may be changed between steps (a replayed step keeps those of its capture).
-    Parameters whose gradient is None are left as they are."""
+    Parameters whose gradient is None are left as they are.  Not made inside a graph capture."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
                  master_weights=False, max_grad_norm=None, seed=0):
         params = list(params)
         _check_tensors(params, "params")
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("AdamW: its states and table would hold nothing before the graph's first replay; make it before the capture")
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits={state_bits!r}: 32 or 8")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):

@@ -530,3 +530,15 @@ def test_values_changed_between_steps_count(bits):
             opt.step(make(sizes, torch.float32, 1))
         setattr(opt, name, keep)
     assert opt.step_count == 1 + len(changes)
+
+
+def test_an_optimizer_is_not_made_in_a_capture():
+    from muzero_amd.optim import AdamW
+    p = torch.ones(70, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="before the capture"):
+            AdamW([p])
+        p.mul_(2.0)
+    graph.replay()
+    assert bool((p == 2.0).all())       # the capture went on

@@ -150,3 +150,12 @@ def test_a_cut_call_without_its_workspace_is_refused():
     for given, at in ((0, None), (size.value - 1, 4096), (size.value, None)):
         a.workspace, a.workspace_bytes = at, given
         assert lib.mzs_policy_log_probs(C.byref(a), None) == -1 and b"workspace" in lib.mzs_last_error()
+
+
+def test_what_a_capture_would_leave_unwritten_is_not_made_there(monkeypatch):
+    """Refused before anything is allocated."""
+    monkeypatch.setattr(optim, "_check_tensors", lambda tensors, what: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for make in (optim.AdamW, optim.TensorList):
+        with pytest.raises(ValueError, match="before the capture"):
+            make([torch.zeros(3)])
