@@ -44,10 +44,29 @@ class _Table:
         self.n, self.tiles, self.ptr = n, tiles.value, self.memory.data_ptr()
 
 
+class _Written:
+    """Memory that the current stream has written last, for users on other streams: use() before each."""
+
+    def __init__(self, device, tensors):
+        stream = torch.cuda.current_stream(device)
+        self.device, self.tensors, self._seen = device, tensors, {stream.cuda_stream}
+        self._event = torch.cuda.Event()
+        self._event.record(stream)
+
+    def use(self, raw_stream):
+        if raw_stream not in self._seen:
+            self._event.synchronize()       # once per stream; on the host, so that a capture records nothing of it
+            stream = torch.cuda.current_stream(self.device)
+            for t in self.tensors:          # freed, it is not given out again before that stream's work so far is done
+                t.record_stream(stream)
+            self._seen.add(raw_stream)
+
+
 class TensorList:
     """A list of tensors laid out once for grad_norm and AdamW.step: for gradients that stay in the same buffers from step
-    to step.  The list refers to (and keeps alive) the memory the tensors have now.  Not made inside a graph capture
-    (used inside one it may be)."""
+    to step.  The list refers to (and keeps alive) the memory the tensors have now: gradients that zero_grad() drops and
+    backward() makes anew are not in it.  Not made inside a graph capture; used inside one (grad_norm) it has to live as
+    long as the graph, AdamW.step keeps it itself."""
 
     def __init__(self, tensors):
         tensors = list(tensors)
@@ -58,20 +77,10 @@ class TensorList:
         self.dtype, self.device = tensors[0].dtype, tensors[0].device
         self.counts = tuple(t.numel() for t in tensors)
         self.table = _Table(self.device, [t.data_ptr() for t in tensors], self.counts)
-        # the table is written on this stream: a user on another one waits for it
-        stream = torch.cuda.current_stream(self.device)
-        self._ready = torch.cuda.Event()
-        self._ready.record(stream)
-        self._waited = {stream.cuda_stream}
+        self._written = _Written(self.device, [self.table.memory])
 
     def __len__(self):
         return len(self.counts)
-
-    def _wait(self, raw_stream):
-        if raw_stream not in self._waited:
-            self._ready.synchronize()       # once per stream; on the host, so that a capture records nothing of it
-            self.table.memory.record_stream(torch.cuda.current_stream(self.device))
-            self._waited.add(raw_stream)
 
 
 def grad_norm(grads, scale=1.0):
@@ -80,8 +89,7 @@ def grad_norm(grads, scale=1.0):
     if isinstance(grads, TensorList):
         dev, dtype, table = grads.device, grads.dtype, grads.table
         stream = _lib.raw_stream(dev.index)
-        if stream not in grads._waited:
-            grads._wait(stream)
+        grads._written.use(stream)
     else:
         grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
         _check_tensors(grads, "grads")
@@ -167,6 +175,9 @@ class AdamW:
         if master_weights:
             a.master = self._state["master"].data_ptr()
         a.control_dev = self.control.data_ptr()
+        self._written = _Written(dev, [self.control, self.grad_norm, self._workspace, *self._state.values()])
+        self._params_written = _Written(dev, [self._params_table.memory])
+        self._captured = []     # what graphs read of tables, for as long as this optimizer lives
 
     # ------------------------------------------------------------------ state
     def state_tensors(self):
@@ -232,8 +243,10 @@ class AdamW:
         .grad.  norm: the norm to clip by (a 0-d float32 tensor) where it covers more than these parameters; None: computed
         here when max_grad_norm is set.  grad_scale multiplies the gradients (1 / loss scale).  grad_norm holds the norm."""
         stream = _lib.raw_stream(self.device.index)
-        if isinstance(grads, TensorList) and stream not in grads._waited:
-            grads._wait(stream)
+        self._written.use(stream)
+        if isinstance(grads, TensorList):
+            grads._written.use(stream)
+        capturing = torch.cuda.is_current_stream_capturing()
         table, dtype = self._grad_table(grads)
         pointers = [p.data_ptr() for p in self.params]
         params_table = self._params_table
@@ -243,8 +256,14 @@ class AdamW:
                     _DTYPES[self.params[0].dtype] != self._args.param_dtype):
                 raise ValueError("the parameters' sizes, type or device changed")
             params_table = _Table(self.device, pointers, self.counts)
-            if not torch.cuda.is_current_stream_capturing():    # a table written inside a graph is that graph's alone
+            if not capturing:       # a table written inside a graph is that graph's alone
                 self._params_table, self._pointers = params_table, pointers
+                self._params_written = _Written(self.device, [params_table.memory])
+        else:
+            self._params_written.use(stream)
+        if capturing:
+            read = [t for t in (params_table, grads) if t is self._params_table or isinstance(t, TensorList)]
+            self._captured += [t for t in read if all(t is not c for c in self._captured)]
         a = self._args
         a.n_tiles, a.params_table, a.grads_table = params_table.tiles, params_table.ptr, table.ptr
         a.grad_dtype, a.grad_scale = _DTYPES[dtype], float(grad_scale)

@@ -542,3 +542,76 @@ def test_an_optimizer_is_not_made_in_a_capture():
         p.mul_(2.0)
     graph.replay()
     assert bool((p == 2.0).all())       # the capture went on
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_waits_for_the_stream_that_made_the_optimizer(bits):
+    """States, master weights and table are written on a stream that is busy; the first step runs on another one at once."""
+    from muzero_amd.optim import AdamW, TensorList, grad_norm
+    sizes = [4096 * 30, 77]
+    a, b = make(sizes, torch.bfloat16, 0, scale=1.0), make(sizes, torch.bfloat16, 0, scale=1.0)
+    gs = make(sizes, torch.bfloat16, 1)
+    want = AdamW(b, state_bits=bits, master_weights=True, max_grad_norm=0.5)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(50_000_000)
+        opt, listed = AdamW(a, state_bits=bits, master_weights=True, max_grad_norm=0.5), TensorList(gs)
+        assert not s.query()
+    opt.step(listed)
+    norm = grad_norm(listed)
+    want.step(gs)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and torch.equal(norm, want.grad_norm)
+
+
+def test_memory_of_a_step_on_another_stream_is_marked_as_its(monkeypatch):
+    """A replaced table, and the states of an optimizer that goes: not given out again before that stream is through."""
+    from muzero_amd.optim import AdamW
+    p = make([5000], torch.float32, 0)
+    opt = AdamW(p, max_grad_norm=1.0)
+    g = make([5000], torch.float32, 1)
+    marked = []
+    record = torch.Tensor.record_stream
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: (marked.append((t.data_ptr(), s.cuda_stream)), record(t, s))[1])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    p[0].data = p[0].data.clone()
+    opt.step(g)                                 # a table of the current stream
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        opt.step(g), opt.step(g)
+    s.synchronize()
+    mine = [opt.control, opt.grad_norm, opt._workspace, opt._params_table.memory, *opt.state_tensors().values()]
+    assert sorted(marked) == sorted((t.data_ptr(), s.cuda_stream) for t in mine)
+
+
+def test_a_graph_keeps_the_tables_that_it_reads():
+    """A captured step, then the parameters' storage replaced, an eager step and the list of gradients gone: the graph goes on with the
+    storage that it was captured on."""
+    from muzero_amd.optim import AdamW, TensorList
+    sizes = [5000, 300]
+    p, q = make(sizes, torch.float32, 0), make(sizes, torch.float32, 0)
+    gs = make(sizes, torch.float32, 1)
+    opt, other = AdamW(p), AdamW(q)
+    listed = TensorList(gs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(listed)
+    tables = [opt._params_table.memory.data_ptr(), listed.table.memory.data_ptr()]
+    size = opt._params_table.memory.numel()
+    del listed
+    old = [t.data for t in p]
+    for t in p:
+        t.data = t.data.clone()
+    opt.step(gs)
+    fill = [torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(400)]
+    assert not {t.data_ptr() for t in fill} & set(tables)       # before the graph reads them
+    other.step(gs)
+    assert all(torch.equal(t, u) for t, u in zip(p, q))
+    for _ in range(2):
+        before = [t.clone() for t in p]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, u) for t, u in zip(p, before)) and not any(torch.equal(t, u) for t, u in zip(p, old))
+    assert opt.step_count == 3
