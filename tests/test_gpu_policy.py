@@ -519,3 +519,20 @@ def test_backward_twice_and_of_parts():
     graph, = torch.autograd.grad(out.log_z.sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):                           # once differentiable: refused, not silently wrong
         graph.sum().backward()
+
+
+@pytest.mark.parametrize("shape", [(6, 9), (2, 3, 9), (9,)])
+def test_outputs_are_tensors_of_their_own(shape):
+    """Operations in place that autograd records are taken by each, and change no other."""
+    from muzero_amd.policy import policy_log_probs, policy_log_probs_grad
+    x = torch.randn(shape, device="cuda")
+    g = torch.ones(shape[:-1], device="cuda")
+    for call in (lambda: policy_log_probs(x, top=2), lambda: policy_log_probs_grad(x, grad_entropy=g, top=2)[0]):
+        want, out = call(), call()
+        scale = torch.full((), 2.0, device="cuda", requires_grad=True)
+        for i in (0, 1, 2, 3):
+            out[i].mul_(scale)
+            assert out[i].requires_grad and torch.equal(out[i].detach(), 2 * want[i])
+            assert all(torch.equal(o.detach(), w) and not o.requires_grad for o, w in zip(out[i + 1:], want[i + 1:]))
+        got, = torch.autograd.grad(sum(o.sum() for o in out[:4]), scale)
+        assert torch.allclose(got, sum(w.sum() for w in want[:4]), rtol=1e-5, atol=0)
