@@ -13,6 +13,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 
@@ -43,9 +44,16 @@ def _call(name):
     return f
 
 
+def _no_tangent(*tensors):
+    for t in tensors:
+        if t is not None and unpack_dual(t).tangent is not None:
+            raise ValueError("policy_log_probs: no forward-mode derivatives (a dual tensor); backward ones through the logits")
+
+
 def _check(logits, actions, mask, temperature, top):
     if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
         raise ValueError("logits: a tensor [..., n_actions]")
+    _no_tangent(logits)
     if not logits.is_cuda:
         raise _lib.MzsError("policy_log_probs: logits must be on a GPU (there is no CPU path)")
     if logits.dtype not in _DTYPES:
@@ -215,6 +223,7 @@ def policy_log_probs_grad(logits, actions=None, grad_log_prob=None, grad_entropy
     one call, for coefficients that are known beforehand (advantages over the batch, an entropy bonus): without
     autograd, so it can be captured into a graph.  The coefficients are tensors [...] or None (0).  out: where the
     gradient goes, of the logits' shape and type with dense rows — `logits` itself is allowed and is then overwritten."""
+    _no_tangent(grad_log_prob, grad_entropy, grad_log_z)
     _check(logits, actions, mask, temperature, top)
     lead, dev = logits.shape[:-1], logits.device
     coefficients = [_coefficient(g, name, lead, dev) for g, name in

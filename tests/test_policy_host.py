@@ -159,3 +159,19 @@ def test_what_a_capture_would_leave_unwritten_is_not_made_there(monkeypatch):
     for make in (optim.AdamW, optim.TensorList):
         with pytest.raises(ValueError, match="before the capture"):
             make([torch.zeros(3)])
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor has no requires_grad: without a look for its tangent the call would drop it."""
+    from torch.autograd import forward_ad
+    x, one = torch.zeros(3, 4), torch.ones(3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3, 4))
+        for call in (lambda: policy.policy_log_probs(dual), lambda: policy.policy_log_probs_grad(dual),
+                     lambda: policy.policy_log_probs_grad(x, None, forward_ad.make_dual(one, one)),
+                     lambda: policy.policy_log_probs_grad(x, None, None, forward_ad.make_dual(one, one)),
+                     lambda: policy.policy_log_probs_grad(x, None, None, None, forward_ad.make_dual(one, one))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        with pytest.raises(_lib.MzsError, match="GPU"):     # a tensor without a tangent is none of its business
+            policy.policy_log_probs(x)
