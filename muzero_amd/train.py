@@ -129,8 +129,8 @@ class Trainer:
     """Owns the training state of one engine handle (one GPU)."""
 
     def __init__(self, engine, unroll_steps, max_batch, optimizer="adam", learning_rate=1e-3,
-                 lr_scheduler=None, num_of_epoch=300, loss_type="general", weight_decay=0.01, max_grad_norm=None):
-        """weight_decay, max_grad_norm: of optimizer="adamw" (muzero_amd.optim.AdamW's rule on the model's weights: decoupled
+                 lr_scheduler=None, num_of_epoch=300, loss_type="general", weight_decay=None, max_grad_norm=None):
+        """weight_decay (0.01), max_grad_norm (none): of optimizer="adamw" alone (muzero_amd.optim.AdamW's rule on the model's weights: decoupled
         decay, the gradient clipped to max_grad_norm, a step whose norm is not finite skipped; the norm is the all-reduced
         gradient's, the same on every rank)."""
         if loss_type not in LOSS_TYPES:
@@ -139,8 +139,8 @@ class Trainer:
             raise ValueError(f"optimizer={optimizer!r}: 'adam' or 'sgd' (muzero_model.py:418-421), or 'adamw'")
         if max_grad_norm is not None and (optimizer != "adamw" or not max_grad_norm > 0.0):
             raise ValueError(f"max_grad_norm={max_grad_norm!r}: positive, with optimizer='adamw'")
-        if optimizer == "adamw" and not 0.0 <= weight_decay < math.inf:
-            raise ValueError(f"weight_decay={weight_decay!r}: finite, not negative")
+        if weight_decay is not None and (optimizer != "adamw" or not 0.0 <= weight_decay < math.inf):
+            raise ValueError(f"weight_decay={weight_decay!r}: finite, not negative, with optimizer='adamw'")
         if lr_scheduler not in SCHEDULERS:
             scheduled_lr(lr_scheduler, learning_rate, num_of_epoch, 1)   # raises with the reason
         self.eng = engine
@@ -152,7 +152,8 @@ class Trainer:
         self.loss_type = loss_type
         _lib.check(self.lib.mzs_train_set_loss(engine.h, *LOSS_TYPES[loss_type]), "mzs_train_set_loss")
         if optimizer == "adamw":
-            _lib.check(self.lib.mzs_train_set_adamw(engine.h, 0.999, 1e-8, float(weight_decay), float(max_grad_norm or 0.0)),
+            _lib.check(self.lib.mzs_train_set_adamw(engine.h, 0.999, 1e-8, 0.01 if weight_decay is None else float(weight_decay),
+                                                    float(max_grad_norm or 0.0)),
                        "mzs_train_set_adamw")
         dev, n = engine.device, engine.weight_count()
         self.bucket, self.grad, self.loss = make_bucket(n, self.K, dev)

@@ -175,3 +175,11 @@ def test_forward_mode_derivatives_are_refused():
                 call()
         with pytest.raises(_lib.MzsError, match="GPU"):     # a tensor without a tangent is none of its business
             policy.policy_log_probs(x)
+
+
+@pytest.mark.parametrize("optimizer", ["adam", "sgd"])
+def test_the_trainer_refuses_options_of_another_optimizer(optimizer):
+    from muzero_amd.train import Trainer
+    for kw, word in ((dict(weight_decay=0.1), "weight_decay"), (dict(weight_decay=0.0), "weight_decay"), (dict(max_grad_norm=1.0), "max_grad_norm")):
+        with pytest.raises(ValueError, match=word):
+            Trainer(None, 5, 8, optimizer, **kw)        # before it looks at the engine
