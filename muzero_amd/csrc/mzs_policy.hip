@@ -177,14 +177,6 @@ struct Sum {
     float big, s, t;
 };
 
-__device__ __forceinline__ Sum sum_merge(Sum a, Sum b, float c) {
-    const float big = fmaxf(a.big, b.big);
-    const float da = a.big == big ? 0.0f : fmaxf(c * (a.big - big), kLow);
-    const float db = b.big == big ? 0.0f : fmaxf(c * (b.big - big), kLow);
-    const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
-    return Sum{big, fa * a.s + fb * b.s, fa * (a.t + da * a.s) + fb * (b.t + db * b.s)};
-}
-
 __device__ __forceinline__ int64_t row_action(const Row& p, int64_t r) {
     if (!p.action) return -1;
     return p.action_bytes == 8 ? static_cast<const int64_t*>(p.action)[r] : (int64_t)static_cast<const int32_t*>(p.action)[r];
