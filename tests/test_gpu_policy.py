@@ -536,3 +536,15 @@ def test_outputs_are_tensors_of_their_own(shape):
             assert all(torch.equal(o.detach(), w) and not o.requires_grad for o, w in zip(out[i + 1:], want[i + 1:]))
         got, = torch.autograd.grad(sum(o.sum() for o in out[:4]), scale)
         assert torch.allclose(got, sum(w.sum() for w in want[:4]), rtol=1e-5, atol=0)
+
+
+@pytest.mark.parametrize("places", [2, 3, 4, 6, 8, 12, 16, 20, 22, 24])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_a_block_on_both_sides_of_each_step(places, dtype):
+    """Rows that fill so many vectors a thread of a block's 512, one logit fewer and one more (an odd start in every second row)."""
+    full = 512 * places * (4 if dtype is torch.float32 else 8)
+    for n in (full - 1, full, full + 1):
+        x, a, m = head(3, n, dtype, n)
+        a[0], a[1] = 0, n - 1
+        m[:2, 0], m[:2, -1] = True, True
+        check(x, a, m, 0.9, top=0)
