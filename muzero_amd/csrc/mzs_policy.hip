@@ -420,7 +420,7 @@ __device__ __forceinline__ void write_best(const Row& p, int64_t r, int lane, co
 
 /* ------------------------------------------------------------------ narrow rows
  * Up to 8 logits: a lane a row, in registers; one read, one write, nothing shared.  Bound by memory: 2M x 4 fp32 with the best action
- * 22 us, 4.1 TB/s of what it reads and writes; 4096 rows 3.3 us, of which an empty launch is 2.5. */
+ * 20 us, 4.5 TB/s of what it reads and writes; 4096 rows 3.3 us, of which an empty launch is 2.5. */
 template <typename T, int E, bool kForward, bool kGrad, bool kTop>
 __global__ void __launch_bounds__(kBlock) k_policy_lanes(const Row p) {
     const int n = (int)p.n;
@@ -732,9 +732,10 @@ __device__ void select_top(const Row& p, int64_t r, const T* l, const uint8_t* m
 
 /* Forward pass of a chunk: one read, running maximum and sums, four vectors a thread on their way while four are summed.  kSplit: the
  * chunk's part goes to parts[row][chunk] and its strips' maxima to strips[row][chunk][strip]; else the chunk is the row.  Bound by the read
- * and, beside it, by the arithmetic (an element's exponential and eight more operations take half the time of its read): 640 x 100000 bf16
- * from memory 30 us, 4.2 TB/s, 39 with the five best alternatives, whose search every block ends with at once; two vectors in flight 30,
- * six 33, at least six waves a SIMD (fewer registers) 33. */
+ * and the arithmetic alike: an element's eight operations and its exponential, which takes four places, are 19.5 us of the card's lanes for 64M
+ * elements, the read of 640 x 100000 bf16 19.7, and with 2.5 waves a SIMD the two overlap in part: 30 to 34 us from memory, 4.2 TB/s, 37 to 39
+ * with the five best alternatives, whose search every block ends with at once; two vectors in flight 30, six 33, at least six waves a SIMD
+ * (fewer registers) 33. */
 template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kBlock) k_policy_chunk(const Row p, int chunks, int chunk_vecs, float* __restrict__ parts,
                                                          float* __restrict__ strips) {

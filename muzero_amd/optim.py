@@ -85,7 +85,7 @@ class TensorList:
 
 def grad_norm(grads, scale=1.0):
     """sqrt of the sum of squares over all gradients, times |scale|: a 0-d float32 tensor, summed in fp64 in a fixed order.
-    grads: a tensor, a list of tensors of one type (None: left out), or a TensorList."""
+    grads: a tensor, a list of tensors of one type (None: left out), or a TensorList.  No gradient flows through it."""
     if isinstance(grads, TensorList):
         dev, dtype, table = grads.device, grads.dtype, grads.table
         stream = _lib.raw_stream(dev.index)
