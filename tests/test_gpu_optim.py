@@ -615,3 +615,36 @@ def test_a_graph_keeps_the_tables_that_it_reads():
         torch.cuda.synchronize()
         assert all(torch.equal(t, u) for t, u in zip(p, before)) and not any(torch.equal(t, u) for t, u in zip(p, old))
     assert opt.step_count == 3
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_elements_past_32_bits(bits):
+    """One tensor of 2^32 + 5000 elements, zeros but for parts on both sides of 2^31 and 2^32 and at its ends: each part as a short tensor's
+    own step (8 bits: those whose elements' numbers are equal in 32 bits, which is what the dither takes of them)."""
+    from muzero_amd.optim import AdamW, grad_norm
+    n, part = 2 ** 32 + 5000, 5000
+    starts = [0, 2 ** 31 - 2500, 2 ** 32 - 5000, 2 ** 32]
+    w, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    ws, gs = make([part] * 4, torch.bfloat16, 1, scale=1.0), make([part] * 4, torch.bfloat16, 2)
+    for at, a, b in zip(starts, ws, gs):
+        w[at:at + part], g[at:at + part] = a, b
+    norm = grad_norm([g])
+    want = math.sqrt(sum((b.double() ** 2).sum().item() for b in gs))
+    assert abs(float(norm) - want) <= 4 * U * want
+    opt = AdamW([w], lr=0.01, state_bits=bits, max_grad_norm=0.5, seed=5)
+    for _ in range(2):
+        opt.step([g])
+    state = opt.state_tensors()
+    for at, a, b in zip(starts, ws, gs):
+        if bits == 8 and at % 2 ** 32:
+            continue
+        short = AdamW([a], lr=0.01, state_bits=bits, max_grad_norm=0.5, seed=5)
+        for _ in range(2):
+            short.step([b], norm=norm)
+        assert torch.equal(w[at:at + part], a)
+        for k, v in short.state_tensors().items():
+            each = 32 if "exponent" in k else 1
+            got = state[k].view(torch.uint8).view(v.dtype)[at // each:at // each + part // each]
+            assert torch.equal(got.view(torch.uint8), v[:part // each].view(torch.uint8))
+    quiet = w[2 ** 31 + 2500:2 ** 32 - 5000]
+    assert not bool(quiet.any())

@@ -110,3 +110,42 @@ def test_a_block_a_row_for_more_rows_than_blocks_of_a_launch():
     out = policy_log_probs(x, a, top=1)
     check_rows(torch.cat([at_borders(rows, 2 ** 20), at_borders(rows, 2 ** 24)]), x, a, None, 1.0, 1, out)
     assert bool((out.log_z == out.log_z[0]).all()) and bool((out.top_action == out.top_action[0]).all())
+
+
+@pytest.mark.parametrize("n, odd", [(2 ** 28, 0), (2 ** 28 - 3, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_widest_row(n, odd, dtype):
+    """2^28 logits, cut over 256 blocks of 256 threads: q = n / 65536 + 40 roundings one after the other in a sum, in the notation of
+    test_gpu_policy; alternatives and the action near the row's end."""
+    from muzero_amd.policy import policy_log_probs, policy_log_probs_grad
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(n + odd, generator=g, device="cuda").to(dtype)[odd:][None]
+    best = torch.cat([torch.arange(n - 20, n), torch.tensor([0, 1, 2 ** 27, 2 ** 27 + 1]), torch.arange(2 ** 20, 2 ** 20 + 8)]).cuda()
+    x[0, best] = 12.0 - torch.arange(32, device="cuda").to(dtype) / 8       # exact, apart from each other and from the rest
+    a = torch.tensor([n - 2], device="cuda")
+    up = [torch.full((1,), c, device="cuda") for c in (0.7, -0.3, 0.2)]
+    out = policy_log_probs(x, a, top=32)
+    both, grad = policy_log_probs_grad(x, a, *up)
+    z = x[0].double()
+    d = z - 12.0
+    p = torch.exp(d)
+    s = float(p.sum())
+    p /= s
+    D1, D2 = float((p * -d).sum()), float((p * d * d).sum())
+    log_z, h = 12.0 + np.log(s), float(np.log(s)) + D1
+    q = n / 65536 + 40
+    for o in (out, both):
+        assert abs(float(o.log_z) - log_z) <= q * U + 3 * U * D1 + 3 * U * 12
+        assert abs(float(o.entropy) - h) <= (q + 4) * U * (1 + D1) + 3 * U * (D1 + D2)
+        assert abs(float(o.log_prob) - float(z[n - 2] - log_z)) <= q * U + 3 * U * (D1 + 60)
+    assert torch.equal(out.top_action[0].long(), best)
+    logp = d - np.log(s)
+    k = 0.2 - 0.7 + 0.3 * (logp + h)
+    size = 0.9 + 0.3 * (logp.abs() + h)
+    want = p * k
+    tol = p * size * U * (q + 8 + 3 * (logp.abs() + 2 * D1 + 1)) + p * 0.3 * 2 * ((q + 4) * U * (1 + D1) + 3 * U * (D1 + D2 + 12))
+    want[n - 2] += 0.7
+    tol[n - 2] += 4 * U * 0.7
+    tol += (want.abs() + tol) * torch.finfo(dtype).eps / 2 + 2.0 ** -125
+    off = (grad[0].double() - want).abs()
+    assert bool((off <= tol).all()), (int((off > tol).sum()), float((off / tol).max()))
